@@ -28,6 +28,7 @@ from .ops.mx import (mxf8_matmul, mxf8_matmul_reduce_scatter, quantize_mxf8, deq
 
 from .ops.attention import flash_attention  # noqa: F401
 from .ops.mla import mla_decode  # noqa: F401
+from .ops.kv4 import kv4_cache, kv4_append, kv4_read, kv4_decode, kv4_evict  # noqa: F401
 
 from .ops import torch_ops  # noqa: F401  (registers torch.ops.catcoc.*)
 

@@ -52,6 +52,8 @@ SOURCES = [
     "kernels/flash_decode.cu",
     "kernels/mla_decode.cu",
     "kernels/mla_rows.cu",
+    "kernels/kv4_cache.cu",
+    "kernels/kv4_decode.cu",
     "shmem/host.cu",
     "oracle/oracle.cpp",
 ]

@@ -184,6 +184,12 @@ def _declare(lib) -> None:
         "catcoc_mla_decode": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, i32, vp, u64, vp]),
         "catcoc_mla_rows_workspace_bytes": (i64, [i32, i32, i32, i32]),
         "catcoc_mla_rows": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, u64, vp]),
+        "catcoc_kv4_block_bytes": (i64, [i32]),
+        "catcoc_kv4_append": (i32, [vp, vp, i64, i64, vp, i64, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp]),
+        "catcoc_kv4_read": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp]),
+        "catcoc_kv4_evict": (i32, [vp] * 8 + [i32] * 11 + [vp, vp]),
+        "catcoc_kv4_decode_workspace_bytes": (i64, [i32] * 9),
+        "catcoc_kv4_decode": (i32, [vp, vp, vp, vp, vp, vp, i64, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, u64, vp]),
         "catcoc_matmul_noalloc": (i32, [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, i32, vp]),
         "catcoc_matmul_noalloc_status": (i32, [P(u32)]),
     }

@@ -365,6 +365,31 @@ int catcoc_mla_rows(const void* q_nope, const void* q_rope, const void* ckv, con
                     const int* kv_lens, void* out, void* workspace, int B, int q_len, int H, int num_pages, int max_pages,
                     int fmt, int causal, float scale, uint32_t* status, uint64_t timeout_ns, void* stream);
 
+/* ---- paged key / value cache in 4 bits (csrc/kernels/kv4_cache.cu, kv4_decode.cu; layout: kv4.h) ----
+ * cache: uint8 [pages, Hk, catcoc_kv4_block_bytes(D)], 64 tokens of a head a block, D = 64 or 128; block_table [B, max_pages] and
+ * kv_lens [B] are device int32. A page outside the cache or a length outside the table's row is noted in `status` and left out. */
+int64_t catcoc_kv4_block_bytes(int D);
+/* Quantises T new tokens (fp16 / bf16; a token's and a head's pitch in elements, multiples of 8) into the cache. Sequence b has the
+ * tokens [ends[b - 1], ends[b]), or T / B each without `ends`; its last token stands at kv_lens[b] - 1. Tokens from ends[B - 1] on are left out. */
+int catcoc_kv4_append(void* cache, const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
+                      const int* block_table, const int* kv_lens, const int* ends, int T, int B, int Hk, int D, int pages, int max_pages,
+                      int fmt, uint32_t* status, void* stream);
+/* k, v [B, Hk, count, D]: the values at the positions [start[b], start[b] + count) (from 0 without `start`), zero outside the sequence */
+int catcoc_kv4_read(const void* cache, const int* block_table, const int* kv_lens, const int* start, void* k, void* v, int B, int Hk, int D,
+                    int pages, int max_pages, int count, int fmt, uint32_t* status, void* stream);
+/* Cuts every sequence to its first `sinks`, last `recent` and, of the others, heaviest tokens (the first ones of equal weight), `keep`
+ * in all, in order. kept [B, Hk, keep] (-1 behind the last), out_lens [B], out_weights [B, Hk, S_out] (zero behind the last).
+ * In place when out_table is block_table. Two launches. */
+int catcoc_kv4_evict(void* cache, const float* weights, float* out_weights, const int* block_table, const int* out_table, const int* kv_lens,
+                     int* kept, int* out_lens, int B, int Hk, int D, int pages, int max_pages, int out_pages, int S, int S_out, int keep,
+                     int recent, int sinks, uint32_t* status, void* stream);
+/* Attention of q_len new tokens of every sequence (q, out [B * q_len, Hq, D]); token t sees the keys up to its own, with window > 0 of
+ * those the last `window` and the first `sinks`. weights (fp32, B * Hk rows of weights_pitch) += the probabilities of a KV head's rows. */
+int64_t catcoc_kv4_decode_workspace_bytes(int B, int q_len, int Hq, int Hk, int D, int max_pages, int window, int sinks, int weights);
+int catcoc_kv4_decode(const void* q, const void* cache, const int* block_table, const int* kv_lens, void* out, float* weights,
+                      int64_t weights_pitch, void* workspace, int B, int q_len, int Hq, int Hk, int D, int pages, int max_pages, int window,
+                      int sinks, int fmt, float scale, uint32_t* status, uint64_t timeout_ns, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
