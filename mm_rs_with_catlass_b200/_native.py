@@ -180,6 +180,9 @@ def _declare(lib) -> None:
         "catcoc_flash_attention_cut": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, u64, vp]),
         "catcoc_flash_decode_workspace_bytes": (i64, [i32, i32, i32, i32, i32, i32]),
         "catcoc_flash_decode": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, u64, vp]),
+        "catcoc_window_route": (i64, [i32] * 8),
+        "catcoc_window_attention": (i32, [vp, vp, vp, vp, vp] + [i32] * 9 + [C.c_float, vp, u64, vp]),
+        "catcoc_window_decode_workspace_bytes": (i64, [i32] * 8),
         "catcoc_mla_workspace_bytes": (i64, [i32, i32, i32, i32]),
         "catcoc_mla_decode": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, i32, vp, u64, vp]),
         "catcoc_mla_rows_workspace_bytes": (i64, [i32, i32, i32, i32]),

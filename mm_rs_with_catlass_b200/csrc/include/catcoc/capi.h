@@ -346,6 +346,16 @@ int catcoc_flash_decode(const void* q, const void* k, const void* v, void* out, 
  * -1 - n bytes. */
 int64_t catcoc_attention_route(int B, int Hq, int Hk, int Sq, int Sk, int D, int causal);
 
+/* Causal attention with a sliding window: position p = i + (Sk - Sq) sees the keys j <= p with p - j < window or j < sinks (window >= 1,
+ * sinks >= 0); blocks of keys that no row of a tile sees are not visited. catcoc_window_route: scratch, n >= 0 or -1 - n bytes as above; catcoc_window_attention
+ * takes either kernel. catcoc_window_decode*: the few-rows kernel by itself. */
+int64_t catcoc_window_route(int B, int Hq, int Hk, int Sq, int Sk, int D, int window, int sinks);
+int catcoc_window_attention(const void* q, const void* k, const void* v, void* out, void* workspace, int B, int Hq, int Hk, int Sq, int Sk, int D,
+                            int fmt, int window, int sinks, float scale, uint32_t* status, uint64_t timeout_ns, void* stream);
+int64_t catcoc_window_decode_workspace_bytes(int B, int Hq, int Hk, int Sq, int Sk, int D, int window, int sinks);
+int catcoc_window_decode(const void* q, const void* k, const void* v, void* out, void* workspace, int B, int Hq, int Hk, int Sq, int Sk, int D,
+                         int fmt, int window, int sinks, float scale, uint32_t* status, uint64_t timeout_ns, void* stream);
+
 /* ---- multi-head latent attention, decode step over a paged cache (csrc/kernels/mla_decode.cu) ----
  * q_nope [T, H, 512], q_rope [T, H, 64] (T = B * q_len new tokens, q_len 1..4), latent cache [num_pages, 128, 512],
  * rotary cache [num_pages, 128, 64], block_table [B, max_pages] and kv_lens [B] (device int32), out [T, H, 512]; all

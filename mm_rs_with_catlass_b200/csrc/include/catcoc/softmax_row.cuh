@@ -24,6 +24,14 @@ CATCOC_DEVICE uint32_t pack16(float lo, float hi) {
   else { __half2 hh = __floats2half2_rn(lo, hi); return *reinterpret_cast<uint32_t*>(&hh); }
 }
 
+// Which scores of a block a row does not see: those from key `vis_left` on, or, with a window, also those in front of its first key
+// that are none of the first `sinks` (all counted from the block's first key).
+struct WindowMask {
+  int vis_left, first, sinks;
+};
+CATCOC_DEVICE bool hides(int vis_left, int i) { return i >= vis_left; }
+CATCOC_DEVICE bool hides(const WindowMask& w, int i) { return i >= w.vis_left || (i < w.first && i >= w.sinks); }
+
 // m: reference maximum (log2 domain), l: running sum
 struct RowState {
   float m = -INFINITY, l = 0.0f;
@@ -47,12 +55,12 @@ CATCOC_DEVICE void rescale_o(uint32_t t_o, float alpha) {
 // place, and updates the state. `loaded()` is called when the scores are in registers, `before(move, alpha)` ahead of the
 // first probability: with `move` (the same in all lanes) the reference maximum of some row of the warp moved and O has to
 // be multiplied by alpha; `ready()` ahead of the first store of probabilities, `half()` behind
-// it (those of the first 64 keys). `vis_left`: keys of this block the row sees (used when `masked`).
+// it (those of the first 64 keys). `mask`: the keys of this block the row sees (used when `masked`), a number of them or a WindowMask.
 //
 // Tried and not kept: a quarter of the exponentials as a degree-5 polynomial on the FMA pipe (D = 128, causal 4 % faster, not causal 2
 // to 6 % slower, D = 64 slower), the two warps of a scheduler taking their exponentials strictly in turn (4 % slower).
-template <int FMT, class Loaded, class Before, class Ready, class Half>
-CATCOC_DEVICE void softmax_row_block(uint32_t t_s, uint32_t t_p, bool masked, int vis_left, float sc, RowState& st, Loaded&& loaded,
+template <int FMT, class Mask, class Loaded, class Before, class Ready, class Half>
+CATCOC_DEVICE void softmax_row_block(uint32_t t_s, uint32_t t_p, bool masked, Mask mask, float sc, RowState& st, Loaded&& loaded,
                                      Before&& before, Ready&& ready, Half&& half) {
   uint32_t v[4][32];
 #pragma unroll
@@ -64,7 +72,7 @@ CATCOC_DEVICE void softmax_row_block(uint32_t t_s, uint32_t t_p, bool masked, in
     for (int c = 0; c < 4; ++c)
 #pragma unroll
       for (int i = 0; i < 32; ++i)
-        if (c * 32 + i >= vis_left) v[c][i] = 0xff800000u;   // -inf: its probability is exactly zero
+        if (hides(mask, c * 32 + i)) v[c][i] = 0xff800000u;   // -inf: its probability is exactly zero
   }
   float mx[4];
 #pragma unroll

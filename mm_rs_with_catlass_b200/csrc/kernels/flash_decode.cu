@@ -19,7 +19,9 @@
 // Roles of the reference this kernel plays (different construction, same jobs):
 //   3rdparty/catlass/include/catlass/gemm/block/block_mmad_fa_qk.hpp, block_mmad_fa_pv.hpp
 //   3rdparty/catlass/include/catlass/epilogue/block/block_epilogue_fa_softmax.hpp, ..._fa_rescale_o.hpp
+#include <algorithm>
 #include <cstring>
+#include <type_traits>
 #include "catcoc/attn_host.h"
 #include "catcoc/capi.h"
 #include "catcoc/host_util.h"
@@ -53,6 +55,8 @@ struct DecodeParams {
   int nb;                         // key blocks per sequence
   int per;                        // key blocks per CTA
   int causal;                     // key j is visible to row r when j <= r % Sq + (Sk - Sq)
+  int window, sinks;              // WINDOW: of those the last `window` and the first `sinks`
+  int sink_blocks, first;         // ... so that a sequence's list is its first blocks and those from `first` on
   float scale_log2;               // softmax scale * log2(e), > 0
   uint32_t idesc_qk, idesc_pv;
   uint32_t* status;
@@ -78,7 +82,7 @@ CATCOC_DEVICE void fail(const DecodeParams& p, uint32_t what, uint32_t a, uint32
 CATCOC_HD int item_of_k(int i) { return i == 0 ? 0 : 2 * i - 1; }
 CATCOC_HD int item_of_v(int i, int n) { return i + 1 < n ? 2 * i + 2 : 2 * n - 1; }
 
-template <int D, int FMT>
+template <int D, int FMT, bool WINDOW>
 __global__ void __launch_bounds__(kThreads, 1) flash_decode_kernel(const __grid_constant__ DecodeParams p) {
   constexpr int kDB = D / 64;                    // 128-byte blocks along the head dimension
   constexpr int kQBytes = kDB * kBlockBytes;
@@ -96,6 +100,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_decode_kernel(const __grid_
   const int g_begin = blockIdx.x * p.per;                       // this CTA's run of the block list
   const int n_run = min(total, g_begin + p.per) - g_begin;      // > 0: the grid covers the list exactly
   const int row_warps = (p.rows + 31) / 32;                     // softmax warps per group that own rows
+  auto block_of = [&](int i) { return WINDOW && i >= p.sink_blocks ? p.first + i - p.sink_blocks : i; };
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -147,7 +152,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_decode_kernel(const __grid_
       if (ptx::elect_one()) {
         ptx::mbar_expect_tx(&bars->kv_full[slot], kSlotBytes);
         for (int d = 0; d < kDB; ++d)
-          ptx::tma_load_3d(skv + slot * kSlotBytes + d * kBlockBytes, is_k ? &p.tm_k : &p.tm_v, &bars->kv_full[slot], d * 64, blk * kBKV, bh);
+          ptx::tma_load_3d(skv + slot * kSlotBytes + d * kBlockBytes, is_k ? &p.tm_k : &p.tm_v, &bars->kv_full[slot], d * 64, block_of(blk) * kBKV, bh);
       }
       __syncwarp();
     }
@@ -239,8 +244,14 @@ __global__ void __launch_bounds__(kThreads, 1) flash_decode_kernel(const __grid_
       for (int i = mine0; i < i1; i += 2) {
         if (!ptx::mbar_wait(&bars->s_full[t], static_cast<uint32_t>(i >> 1) & 1u, p.timeout_ns, abort_flag)) { ok = false; break; }
         ptx::tcgen05_fence_after();
-        const int key0 = (blk0 + i - i0) * kBKV;
-        attn::softmax_row_block<FMT>(t_s, t_s, key0 + kBKV > vis_all, vis - key0, p.scale_log2, st, [] {}, [&](bool move, float alpha) {
+        const int key0 = block_of(blk0 + i - i0) * kBKV;
+        bool masked = key0 + kBKV > vis_all;
+        if constexpr (WINDOW) masked = masked || (key0 <= p.Sk - 1 - p.window && key0 + kBKV > p.sinks);
+        auto mask = [&] {
+          if constexpr (WINDOW) return attn::WindowMask{vis - key0, vis - p.window - key0, p.sinks - key0};   // (vis - 1 is the row's position)
+          else return vis - key0;
+        }();
+        attn::softmax_row_block<FMT>(t_s, t_s, masked, mask, p.scale_log2, st, [] {}, [&](bool move, float alpha) {
           // s_full(i) was committed behind the second product of this parity's previous block, so O_t is whole
           if (move && i > mine0) attn::rescale_o<D>(t_o, alpha);
         }, [] {}, [] {});
@@ -373,17 +384,23 @@ namespace {
 struct DecodePlan {
   int rows = 0, nb = 0, per = 0, ctas = 0;
   bool cut = false;              // some sequence is spread over several CTAs
+  int sink_blocks = 0, first = 0;   // a window leaves out the blocks between them
 };
 
 // Runs of equal length over all SMs. A run is a whole number of sequences where that costs no more than two blocks
 // (a block is about 1.4 us of one SM's share of the bandwidth, the second kernel and its workspace about two of them), or where
 // the whole run is short: a second launch costs the caller more than the blocks (8 x 4 KV heads, 2 tokens, 700 keys 20.7 -> 15.7
 // us, 4 x 4, 1 token, 576 keys 19.8 -> 15.8 with D = 64).
-DecodePlan decode_plan(int B, int Hq, int Hk, int Sq, int Sk, int sms) {
+DecodePlan decode_plan(int B, int Hq, int Hk, int Sq, int Sk, int sms, int window = 0, int sinks = 0) {
   DecodePlan d;
   const int64_t bh = static_cast<int64_t>(B) * Hk;
   d.rows = Hq / Hk * Sq;
   d.nb = (Sk + decode::kBKV - 1) / decode::kBKV;
+  if (window > 0) {
+    d.first = std::max(0, Sk - Sq - window + 1) / decode::kBKV;
+    d.sink_blocks = std::min((sinks + decode::kBKV - 1) / decode::kBKV, d.first);
+    d.nb -= d.first - d.sink_blocks;
+  }
   const int64_t total = bh * d.nb;
   int64_t per = (total + sms - 1) / sms;
   if (per < 2) per = 2;                                     // both softmax groups have work
@@ -403,21 +420,28 @@ int device_sms() {
 }  // namespace
 
 // Does the few-rows kernel take this call, and with how much workspace? (-1: no)
-extern "C" int64_t catcoc_flash_decode_workspace_bytes(int B, int Hq, int Hk, int Sq, int Sk, int D) {
+static int64_t decode_scratch(int B, int Hq, int Hk, int Sq, int Sk, int D, int window, int sinks) {
   if (B <= 0 || Hq <= 0 || Hk <= 0 || Sq <= 0 || Sk <= 0 || Hq % Hk != 0 || (D != 64 && D != 128)) return -1;
   // The query rows of a KV head fill at most one tile of 128: the general kernel spends two tiles per query HEAD on them.
   if (static_cast<int64_t>(Hq / Hk) * Sq > decode::kRows) return -1;
   if (static_cast<int64_t>(B) * Hk * ((Sk + decode::kBKV - 1) / decode::kBKV) > (1ll << 30)) return -1;
-  const DecodePlan d = decode_plan(B, Hq, Hk, Sq, Sk, device_sms());
+  const DecodePlan d = decode_plan(B, Hq, Hk, Sq, Sk, device_sms(), window, sinks);
   if (!d.cut) return 0;
   return (static_cast<int64_t>(d.ctas) + static_cast<int64_t>(B) * Hk) * d.rows * (D + 2) * static_cast<int64_t>(sizeof(float));
 }
 
-extern "C" int catcoc_flash_decode(const void* q, const void* k, const void* v, void* out, void* workspace, int B, int Hq,
-                                   int Hk, int Sq, int Sk, int D, int fmt, int causal, float scale, uint32_t* status,
-                                   uint64_t timeout_ns, void* stream_) {
+extern "C" int64_t catcoc_flash_decode_workspace_bytes(int B, int Hq, int Hk, int Sq, int Sk, int D) {
+  return decode_scratch(B, Hq, Hk, Sq, Sk, D, 0, 0);
+}
+
+extern "C" int64_t catcoc_window_decode_workspace_bytes(int B, int Hq, int Hk, int Sq, int Sk, int D, int window, int sinks) {
+  return Sk < Sq || window < 1 || sinks < 0 ? -1 : decode_scratch(B, Hq, Hk, Sq, Sk, D, std::min(window, 1 << 30), std::min(sinks, 1 << 30));
+}
+
+static int decode_call(const void* q, const void* k, const void* v, void* out, void* workspace, int B, int Hq, int Hk, int Sq, int Sk, int D, int fmt,
+                       int causal, float scale, uint32_t* status, uint64_t timeout_ns, void* stream_, int window, int sinks) {
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  const int64_t need = catcoc_flash_decode_workspace_bytes(B, Hq, Hk, Sq, Sk, D);
+  const int64_t need = decode_scratch(B, Hq, Hk, Sq, Sk, D, window, sinks);
   if (!q || !k || !v || !out || !status || need < 0 || (need > 0 && workspace == nullptr)) {
     set_error("flash_decode: bad arguments");
     return CATCOC_E_BAD_ARG;
@@ -425,7 +449,7 @@ extern "C" int catcoc_flash_decode(const void* q, const void* k, const void* v, 
   if (fmt != CATCOC_FMT_F16 && fmt != CATCOC_FMT_BF16) { set_error("flash_attention takes fp16 / bf16"); return CATCOC_E_UNSUPPORTED; }
   if (causal && Sk < Sq) { set_error("causal attention needs Sk >= Sq"); return CATCOC_E_BAD_ARG; }
   if (!(scale > 0.0f)) { set_error("flash_attention: the softmax scale must be positive (the row maximum is taken before scaling)"); return CATCOC_E_UNSUPPORTED; }
-  const DecodePlan d = decode_plan(B, Hq, Hk, Sq, Sk, device_sms());
+  const DecodePlan d = decode_plan(B, Hq, Hk, Sq, Sk, device_sms(), window, sinks);
   decode::DecodeParams p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType dt = fmt == CATCOC_FMT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
@@ -441,6 +465,7 @@ extern "C" int catcoc_flash_decode(const void* q, const void* k, const void* v, 
     p.part_ml = p.part_o + (static_cast<int64_t>(d.ctas) + bh) * d.rows * D;
   }
   p.causal = causal ? 1 : 0;
+  p.window = window; p.sinks = sinks; p.sink_blocks = d.sink_blocks; p.first = d.first;
   p.scale_log2 = scale * 1.4426950408889634f;
   const uint32_t f = fmt == CATCOC_FMT_BF16 ? 1u : 0u;
   p.idesc_qk = ptx::make_instr_desc(1u, f, f, 0u, 0u, 128u, 128u);
@@ -458,10 +483,25 @@ extern "C" int catcoc_flash_decode(const void* q, const void* k, const void* v, 
     CATCOC_CUDA_OK(launch_overlapped(combine_kernel, grid, dim3(128), 0, stream, p.part_o, p.part_ml, out, p.rows, p.nb, p.per));
     return CATCOC_OK;
   };
-  if (D == 128) {
-    return fmt == CATCOC_FMT_BF16 ? launch(decode::flash_decode_kernel<128, FMT_BF16>, decode::flash_combine_kernel<128, FMT_BF16>)
-                                  : launch(decode::flash_decode_kernel<128, FMT_F16>, decode::flash_combine_kernel<128, FMT_F16>);
-  }
-  return fmt == CATCOC_FMT_BF16 ? launch(decode::flash_decode_kernel<64, FMT_BF16>, decode::flash_combine_kernel<64, FMT_BF16>)
-                                : launch(decode::flash_decode_kernel<64, FMT_F16>, decode::flash_combine_kernel<64, FMT_F16>);
+  auto by_window = [&](auto dim, auto type) -> int {
+    constexpr int kD = decltype(dim)::value, kF = decltype(type)::value;
+    return window > 0 ? launch(decode::flash_decode_kernel<kD, kF, true>, decode::flash_combine_kernel<kD, kF>)
+                      : launch(decode::flash_decode_kernel<kD, kF, false>, decode::flash_combine_kernel<kD, kF>);
+  };
+  using F16 = std::integral_constant<int, FMT_F16>;
+  using BF16 = std::integral_constant<int, FMT_BF16>;
+  if (D == 128) return fmt == CATCOC_FMT_BF16 ? by_window(std::integral_constant<int, 128>{}, BF16{}) : by_window(std::integral_constant<int, 128>{}, F16{});
+  return fmt == CATCOC_FMT_BF16 ? by_window(std::integral_constant<int, 64>{}, BF16{}) : by_window(std::integral_constant<int, 64>{}, F16{});
+}
+
+extern "C" int catcoc_flash_decode(const void* q, const void* k, const void* v, void* out, void* workspace, int B, int Hq,
+                                   int Hk, int Sq, int Sk, int D, int fmt, int causal, float scale, uint32_t* status,
+                                   uint64_t timeout_ns, void* stream) {
+  return decode_call(q, k, v, out, workspace, B, Hq, Hk, Sq, Sk, D, fmt, causal, scale, status, timeout_ns, stream, 0, 0);
+}
+
+extern "C" int catcoc_window_decode(const void* q, const void* k, const void* v, void* out, void* workspace, int B, int Hq, int Hk, int Sq, int Sk, int D,
+                                    int fmt, int window, int sinks, float scale, uint32_t* status, uint64_t timeout_ns, void* stream) {
+  if (window < 1 || sinks < 0) { set_error("window_attention: a window of at least 1 and no negative sinks"); return CATCOC_E_BAD_ARG; }
+  return decode_call(q, k, v, out, workspace, B, Hq, Hk, Sq, Sk, D, fmt, 1, scale, status, timeout_ns, stream, std::min(window, 1 << 30), std::min(sinks, 1 << 30));
 }

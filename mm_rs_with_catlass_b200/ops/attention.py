@@ -28,7 +28,8 @@ from . import _common as cm
 
 
 def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False,
-                    scale: Optional[float] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                    scale: Optional[float] = None, out: Optional[torch.Tensor] = None, window: Optional[int] = None,
+                    sinks: int = 0) -> torch.Tensor:
     """``softmax(scale * q @ k^T [+ causal mask]) @ v`` per (batch, head).
 
     ``q`` is ``[B, Hq, Sq, D]``, ``k`` and ``v`` are ``[B, Hk, Sk, D]`` (fp16 or bf16, ``D`` 64 or
@@ -37,6 +38,10 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
     in the bottom-right corner, as for a decode step over a cache). Scores are accumulated in
     fp32, probabilities are rounded to the operand dtype for the second product, the output is
     rounded once at the end. Returns ``[B, Hq, Sq, D]``.
+
+    With a ``window`` (causal calls) the query at position ``p = i + (Sk - Sq)`` sees of the keys ``j <= p`` only those with
+    ``p - j < window``, and the first ``sinks`` keys, ``j < sinks``, which stay visible to all. The work goes by what is
+    visible: key blocks outside of a tile's windows are not read.
     """
     dev = cm.require_cuda(q, k, v, out)
     if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
@@ -53,6 +58,13 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
         raise ValueError("head dimension %d: 64 and 128 are built" % d)
     if causal and sk < sq:
         raise ValueError("causal attention needs Sk >= Sq")
+    if window is not None:
+        if not causal:
+            raise ValueError("a window needs causal attention")
+        if window < 1 or sinks < 0:
+            raise ValueError("the window must be at least 1 and sinks not negative (got %d and %d)" % (window, sinks))
+    elif sinks:
+        raise ValueError("sinks belong to a window")
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
     if out is None:
         out = torch.empty_like(q)
@@ -64,6 +76,15 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
         raise ValueError("the softmax scale must be positive")
     with cm.guard(dev):
         lib, stream = N.lib(), C.c_void_p(cm.stream_of(dev))
+        if window is not None:
+            window, sinks = min(int(window), 1 << 30), min(int(sinks), 1 << 30)
+            need = int(lib.catcoc_window_route(b, hq, hk, sq, sk, d, window, sinks))
+            need = need if need >= 0 else -1 - need
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            N.check(lib.catcoc_window_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ws.data_ptr() if need else None, b, hq, hk,
+                                                sq, sk, d, cm.out_fmt(q.dtype), window, sinks, float(scale), cm.local_status(dev).data_ptr(),
+                                                cm.default_timeout_ns(), stream))
+            return out
         tail = (b, hq, hk, sq, sk, d, cm.out_fmt(q.dtype), int(causal), float(scale), cm.local_status(dev).data_ptr(),
                 cm.default_timeout_ns(), stream)
         # few query rows per key / value head (decode steps): the keys are cut over the SMs instead of the queries; few tiles of
@@ -76,7 +97,7 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
 
 
 def attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False,
-                        scale: Optional[float] = None) -> torch.Tensor:
+                        scale: Optional[float] = None, window: Optional[int] = None, sinks: int = 0) -> torch.Tensor:
     """The same function in plain fp32 PyTorch (golden for the tests, any device)."""
     b, hq, sq, d = q.shape
     hk, sk = k.shape[1], k.shape[2]
@@ -87,5 +108,6 @@ def attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, ca
     if causal:
         i = torch.arange(sq, device=q.device)[:, None]
         j = torch.arange(sk, device=q.device)[None, :]
-        s = s.masked_fill(j > i + (sk - sq), float("-inf"))
+        p = i + (sk - sq)
+        s = s.masked_fill(j > p if window is None else (j > p) | ((p - j >= window) & (j >= sinks)), float("-inf"))
     return torch.matmul(torch.softmax(s, dim=-1), vf)
