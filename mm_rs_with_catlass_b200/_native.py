@@ -84,6 +84,13 @@ class OpArgs(C.Structure):
     ]
 
 
+class Kv4Call(C.Structure):
+    """Numbers of a call on the 4-bit cache (``CatcocKv4Call``)."""
+    _fields_ = ([(n, C.c_int) for n in ("B", "Hk", "D", "pages", "max_pages", "fmt", "T", "count", "keep", "recent", "out_pages", "S", "S_out", "Hq",
+                                        "q_len", "window", "sinks")] + [("scale", C.c_float)]
+                + [(n, C.c_int64) for n in ("k_token", "k_head", "v_token", "v_head")])
+
+
 class Tile(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("seg", "tile_in_seg", "mi", "ni", "m0", "n0", "rows", "cols")]
 
@@ -188,11 +195,11 @@ def _declare(lib) -> None:
         "catcoc_mla_rows_workspace_bytes": (i64, [i32, i32, i32, i32]),
         "catcoc_mla_rows": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, u64, vp]),
         "catcoc_kv4_block_bytes": (i64, [i32]),
-        "catcoc_kv4_append": (i32, [vp, vp, i64, i64, vp, i64, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp]),
-        "catcoc_kv4_read": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp, vp]),
-        "catcoc_kv4_evict": (i32, [vp] * 8 + [i32] * 11 + [vp, vp]),
-        "catcoc_kv4_decode_workspace_bytes": (i64, [i32] * 9),
-        "catcoc_kv4_decode": (i32, [vp, vp, vp, vp, vp, vp, i64, vp, i32, i32, i32, i32, i32, i32, i32, i32, i32, i32, C.c_float, vp, u64, vp]),
+        "catcoc_kv4_append": (i32, [vp] * 9),
+        "catcoc_kv4_read": (i32, [vp] * 9),
+        "catcoc_kv4_evict": (i32, [vp] * 11),
+        "catcoc_kv4_decode_workspace_bytes": (i64, [vp, i32]),
+        "catcoc_kv4_decode": (i32, [vp] * 9 + [u64, vp]),
         "catcoc_matmul_noalloc": (i32, [vp, i64, vp, i64, vp, i64, i32, i32, i32, i32, i32, i32, i32, vp]),
         "catcoc_matmul_noalloc_status": (i32, [P(u32)]),
     }

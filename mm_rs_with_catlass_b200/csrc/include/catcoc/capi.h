@@ -377,28 +377,39 @@ int catcoc_mla_rows(const void* q_nope, const void* q_rope, const void* ckv, con
 
 /* ---- paged key / value cache in 4 bits (csrc/kernels/kv4_cache.cu, kv4_decode.cu; layout: kv4.h) ----
  * cache: uint8 [pages, Hk, catcoc_kv4_block_bytes(D)], 64 tokens of a head a block, D = 64 or 128; block_table [B, max_pages] and
- * kv_lens [B] are device int32. A page outside the cache or a length outside the table's row is noted in `status` and left out. */
+ * kv_lens [B] are device int32. A page outside the cache or a length outside the table's row is noted in `status` and left out.
+ * The numbers of a call travel in one block, which a caller may keep; each function reads those that it names. */
+typedef struct CatcocKv4Call {
+  int B, Hk, D, pages, max_pages;  /* all */
+  int fmt;                         /* fp16 or bf16 (CATCOC_FMT_*): tokens, values, queries */
+  int T;                           /* append */
+  int count;                       /* read */
+  int keep, recent, out_pages;     /* evict: out_pages: pages in a row of out_table */
+  int S, S_out;                    /* pitch of a head's weights; evict: of its out_weights */
+  int Hq, q_len, window;           /* decode */
+  int sinks;                       /* decode, evict */
+  float scale;                     /* decode */
+  int64_t k_token, k_head, v_token, v_head;   /* append: pitch of a token and of a head in elements, multiples of 8 */
+} CatcocKv4Call;
 int64_t catcoc_kv4_block_bytes(int D);
-/* Quantises T new tokens (fp16 / bf16; a token's and a head's pitch in elements, multiples of 8) into the cache. Sequence b has the
- * tokens [ends[b - 1], ends[b]), or T / B each without `ends`; its last token stands at kv_lens[b] - 1. Tokens from ends[B - 1] on are left out. */
-int catcoc_kv4_append(void* cache, const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
-                      const int* block_table, const int* kv_lens, const int* ends, int T, int B, int Hk, int D, int pages, int max_pages,
-                      int fmt, uint32_t* status, void* stream);
+/* Quantises T new tokens into the cache. Sequence b has the tokens [ends[b - 1], ends[b]), or T / B each without `ends`; its last token
+ * stands at kv_lens[b] - 1. Tokens from ends[B - 1] on are left out. */
+int catcoc_kv4_append(const CatcocKv4Call* c, void* cache, const void* k, const void* v, const int* block_table, const int* kv_lens,
+                      const int* ends, uint32_t* status, void* stream);
 /* k, v [B, Hk, count, D]: the values at the positions [start[b], start[b] + count) (from 0 without `start`), zero outside the sequence */
-int catcoc_kv4_read(const void* cache, const int* block_table, const int* kv_lens, const int* start, void* k, void* v, int B, int Hk, int D,
-                    int pages, int max_pages, int count, int fmt, uint32_t* status, void* stream);
+int catcoc_kv4_read(const CatcocKv4Call* c, const void* cache, const int* block_table, const int* kv_lens, const int* start, void* k, void* v,
+                    uint32_t* status, void* stream);
 /* Cuts every sequence to its first `sinks`, last `recent` and, of the others, heaviest tokens (the first ones of equal weight), `keep`
  * in all, in order. kept [B, Hk, keep] (-1 behind the last), out_lens [B], out_weights [B, Hk, S_out] (zero behind the last).
  * In place when out_table is block_table. Two launches. */
-int catcoc_kv4_evict(void* cache, const float* weights, float* out_weights, const int* block_table, const int* out_table, const int* kv_lens,
-                     int* kept, int* out_lens, int B, int Hk, int D, int pages, int max_pages, int out_pages, int S, int S_out, int keep,
-                     int recent, int sinks, uint32_t* status, void* stream);
+int catcoc_kv4_evict(const CatcocKv4Call* c, void* cache, const float* weights, float* out_weights, const int* block_table, const int* out_table,
+                     const int* kv_lens, int* kept, int* out_lens, uint32_t* status, void* stream);
 /* Attention of q_len new tokens of every sequence (q, out [B * q_len, Hq, D]); token t sees the keys up to its own, with window > 0 of
- * those the last `window` and the first `sinks`. weights (fp32, B * Hk rows of weights_pitch) += the probabilities of a KV head's rows. */
-int64_t catcoc_kv4_decode_workspace_bytes(int B, int q_len, int Hq, int Hk, int D, int max_pages, int window, int sinks, int weights);
-int catcoc_kv4_decode(const void* q, const void* cache, const int* block_table, const int* kv_lens, void* out, float* weights,
-                      int64_t weights_pitch, void* workspace, int B, int q_len, int Hq, int Hk, int D, int pages, int max_pages, int window,
-                      int sinks, int fmt, float scale, uint32_t* status, uint64_t timeout_ns, void* stream);
+ * those the last `window` and the first `sinks`. weights (fp32 [B, Hk, S] or NULL) += the probabilities of a KV head's rows.
+ * catcoc_kv4_decode_workspace_bytes: -1 for a call that is not taken. */
+int64_t catcoc_kv4_decode_workspace_bytes(const CatcocKv4Call* c, int weights);
+int catcoc_kv4_decode(const CatcocKv4Call* c, const void* q, const void* cache, const int* block_table, const int* kv_lens, void* out, float* weights,
+                      void* workspace, uint32_t* status, uint64_t timeout_ns, void* stream);
 
 #ifdef __cplusplus
 }

@@ -379,72 +379,79 @@ int bad(const char* what) {
 
 extern "C" int64_t catcoc_kv4_block_bytes(int D) { return D == 128 ? Block<128>::kBytes : D == 64 ? Block<64>::kBytes : -1; }
 
-extern "C" int catcoc_kv4_append(void* cache, const void* k, int64_t k_token, int64_t k_head, const void* v, int64_t v_token, int64_t v_head,
-                                 const int* block_table, const int* kv_lens, const int* ends, int T, int B, int Hk, int D, int pages,
-                                 int max_pages, int fmt, uint32_t* status, void* stream) {
-  if (!cache || !k || !v || !block_table || !kv_lens || !status || T <= 0 || B <= 0 || Hk <= 0 || pages <= 0 || max_pages <= 0 || (!ends && T % B))
-    return bad("kv4_append: bad arguments");
-  if (D != 64 && D != 128) { set_error("kv4_append: head dimension %d (64 and 128 are built)", D); return CATCOC_E_UNSUPPORTED; }
-  if (fmt != CATCOC_FMT_F16 && fmt != CATCOC_FMT_BF16) { set_error("kv4_append takes fp16 / bf16"); return CATCOC_E_UNSUPPORTED; }
-  if (((reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) || ((k_token | k_head | v_token | v_head) & 7)) {
+namespace {
+// What all calls share; `types`: fp16 and bf16 are told apart
+int common(const CatcocKv4Call* c, const char* what, bool types) {
+  if (!c || c->B <= 0 || c->Hk <= 0 || c->pages <= 0 || c->max_pages <= 0) { set_error("%s: bad arguments", what); return CATCOC_E_BAD_ARG; }
+  if (c->D != 64 && c->D != 128) { set_error("%s: head dimension %d (64 and 128 are built)", what, c->D); return CATCOC_E_UNSUPPORTED; }
+  if (types && c->fmt != CATCOC_FMT_F16 && c->fmt != CATCOC_FMT_BF16) { set_error("%s takes fp16 / bf16", what); return CATCOC_E_UNSUPPORTED; }
+  if (static_cast<int64_t>(c->B) * c->Hk > 0x7fffffff || static_cast<int64_t>(c->max_pages) * kPage > 0x7fffffff) { set_error("%s: too many tokens", what); return CATCOC_E_TOO_LARGE; }
+  return CATCOC_OK;
+}
+bool unaligned(const void* a, const void* b = nullptr, const void* c = nullptr) {
+  return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) & 15) != 0;
+}
+}  // namespace
+
+extern "C" int catcoc_kv4_append(const CatcocKv4Call* c, void* cache, const void* k, const void* v, const int* block_table, const int* kv_lens,
+                                 const int* ends, uint32_t* status, void* stream) {
+  const int rc = common(c, "kv4_append", true);
+  if (rc != CATCOC_OK) return rc;
+  if (!cache || !k || !v || !block_table || !kv_lens || !status || c->T <= 0 || (!ends && c->T % c->B)) return bad("kv4_append: bad arguments");
+  if (unaligned(cache, k, v) || ((c->k_token | c->k_head | c->v_token | c->v_head) & 7)) {
     set_error("kv4_append: rows must begin at 16-byte boundaries");
     return CATCOC_E_ALIGNMENT;
   }
-  const int64_t blocks = (static_cast<int64_t>(T) * Hk * (D / 8) + 255) / 256;
-  if (blocks > 0x7fffffff || static_cast<int64_t>(max_pages) * kPage > 0x7fffffff) { set_error("kv4_append: too many tokens"); return CATCOC_E_TOO_LARGE; }
-  AppendParams p{k, v, k_token, k_head, v_token, v_head, static_cast<uint8_t*>(cache), block_table, kv_lens, ends, T, B, Hk, ends ? 1 : T / B, max_pages, pages, status};
+  const int64_t blocks = (static_cast<int64_t>(c->T) * c->Hk * (c->D / 8) + 255) / 256;
+  if (blocks > 0x7fffffff) { set_error("kv4_append: too many tokens"); return CATCOC_E_TOO_LARGE; }
+  const AppendParams p{k, v, c->k_token, c->k_head, c->v_token, c->v_head, static_cast<uint8_t*>(cache), block_table, kv_lens, ends,
+                       c->T, c->B, c->Hk, ends ? 1 : c->T / c->B, c->max_pages, c->pages, status};
   auto launch = [&](auto kernel) -> int {
     CATCOC_CUDA_OK(launch_overlapped(kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, static_cast<cudaStream_t>(stream), p));
     return CATCOC_OK;
   };
-  if (D == 128) return fmt == CATCOC_FMT_BF16 ? launch(kv4_append_kernel<128, FMT_BF16>) : launch(kv4_append_kernel<128, FMT_F16>);
-  return fmt == CATCOC_FMT_BF16 ? launch(kv4_append_kernel<64, FMT_BF16>) : launch(kv4_append_kernel<64, FMT_F16>);
+  if (c->D == 128) return c->fmt == CATCOC_FMT_BF16 ? launch(kv4_append_kernel<128, FMT_BF16>) : launch(kv4_append_kernel<128, FMT_F16>);
+  return c->fmt == CATCOC_FMT_BF16 ? launch(kv4_append_kernel<64, FMT_BF16>) : launch(kv4_append_kernel<64, FMT_F16>);
 }
 
-extern "C" int catcoc_kv4_read(const void* cache, const int* block_table, const int* kv_lens, const int* start, void* k, void* v, int B, int Hk,
-                               int D, int pages, int max_pages, int count, int fmt, uint32_t* status, void* stream) {
-  if (!cache || !block_table || !kv_lens || !k || !v || !status || B <= 0 || Hk <= 0 || pages <= 0 || max_pages <= 0 || count <= 0)
-    return bad("kv4_read: bad arguments");
-  if (D != 64 && D != 128) { set_error("kv4_read: head dimension %d (64 and 128 are built)", D); return CATCOC_E_UNSUPPORTED; }
-  if (fmt != CATCOC_FMT_F16 && fmt != CATCOC_FMT_BF16) { set_error("kv4_read gives fp16 / bf16"); return CATCOC_E_UNSUPPORTED; }
-  if ((reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) {
-    set_error("kv4_read: buffers must be 16-byte aligned");
-    return CATCOC_E_ALIGNMENT;
-  }
-  const int64_t heads = static_cast<int64_t>(B) * Hk, chunks = (static_cast<int64_t>(count) + 31) / 32;
-  if (heads > 0x7fffffff || chunks > 65535 || static_cast<int64_t>(max_pages) * kPage > 0x7fffffff) { set_error("kv4_read: too many tokens"); return CATCOC_E_TOO_LARGE; }
-  ReadParams p{static_cast<const uint8_t*>(cache), block_table, kv_lens, start, k, v, B, Hk, count, max_pages, pages, status};
+extern "C" int catcoc_kv4_read(const CatcocKv4Call* c, const void* cache, const int* block_table, const int* kv_lens, const int* start, void* k, void* v,
+                               uint32_t* status, void* stream) {
+  const int rc = common(c, "kv4_read", true);
+  if (rc != CATCOC_OK) return rc;
+  if (!cache || !block_table || !kv_lens || !k || !v || !status || c->count <= 0) return bad("kv4_read: bad arguments");
+  if (unaligned(cache, k, v)) { set_error("kv4_read: buffers must be 16-byte aligned"); return CATCOC_E_ALIGNMENT; }
+  const int64_t heads = static_cast<int64_t>(c->B) * c->Hk, chunks = (static_cast<int64_t>(c->count) + 31) / 32;
+  if (chunks > 65535) { set_error("kv4_read: too many tokens"); return CATCOC_E_TOO_LARGE; }
+  const ReadParams p{static_cast<const uint8_t*>(cache), block_table, kv_lens, start, k, v, c->B, c->Hk, c->count, c->max_pages, c->pages, status};
   auto launch = [&](auto kernel) -> int {
     CATCOC_CUDA_OK(launch_overlapped(kernel, dim3(static_cast<unsigned>(heads), static_cast<unsigned>(chunks)), dim3(256), 0, static_cast<cudaStream_t>(stream), p));
     return CATCOC_OK;
   };
-  if (D == 128) return fmt == CATCOC_FMT_BF16 ? launch(kv4_read_kernel<128, FMT_BF16>) : launch(kv4_read_kernel<128, FMT_F16>);
-  return fmt == CATCOC_FMT_BF16 ? launch(kv4_read_kernel<64, FMT_BF16>) : launch(kv4_read_kernel<64, FMT_F16>);
+  if (c->D == 128) return c->fmt == CATCOC_FMT_BF16 ? launch(kv4_read_kernel<128, FMT_BF16>) : launch(kv4_read_kernel<128, FMT_F16>);
+  return c->fmt == CATCOC_FMT_BF16 ? launch(kv4_read_kernel<64, FMT_BF16>) : launch(kv4_read_kernel<64, FMT_F16>);
 }
 
-extern "C" int catcoc_kv4_evict(void* cache, const float* weights, float* out_weights, const int* block_table, const int* out_table, const int* kv_lens,
-                                int* kept, int* out_lens, int B, int Hk, int D, int pages, int max_pages, int out_pages, int S, int S_out, int keep,
-                                int recent, int sinks, uint32_t* status, void* stream_) {
-  if (!cache || !weights || !out_weights || !block_table || !out_table || !kv_lens || !kept || !out_lens || !status || B <= 0 || Hk <= 0 || pages <= 0 ||
-      max_pages <= 0 || out_pages <= 0 || keep <= 0 || recent < 0 || sinks < 0)
+extern "C" int catcoc_kv4_evict(const CatcocKv4Call* c, void* cache, const float* weights, float* out_weights, const int* block_table, const int* out_table,
+                                const int* kv_lens, int* kept, int* out_lens, uint32_t* status, void* stream_) {
+  const int rc = common(c, "kv4_evict", false);
+  if (rc != CATCOC_OK) return rc;
+  if (!cache || !weights || !out_weights || !block_table || !out_table || !kv_lens || !kept || !out_lens || !status || c->out_pages <= 0 || c->keep <= 0 ||
+      c->recent < 0 || c->sinks < 0)
     return bad("kv4_evict: bad arguments");
-  if (D != 64 && D != 128) { set_error("kv4_evict: head dimension %d (64 and 128 are built)", D); return CATCOC_E_UNSUPPORTED; }
-  const int64_t capacity = static_cast<int64_t>(max_pages) * kPage;
-  if (static_cast<int64_t>(recent) + sinks > keep) return bad("kv4_evict: the first and the last tokens are more than what is kept");
-  const int64_t most = std::min<int64_t>(keep, capacity);      // tokens that can stay
-  if (S < capacity || static_cast<int64_t>(out_pages) * kPage < most || S_out < most) return bad("kv4_evict: the weights or the new pages are too short");
-  if (reinterpret_cast<uintptr_t>(cache) & 15) { set_error("kv4_evict: the cache must be 16-byte aligned"); return CATCOC_E_ALIGNMENT; }
-  const int64_t heads = static_cast<int64_t>(B) * Hk;
-  if (heads > 0x7fffffff || capacity > 0x7fffffff) { set_error("kv4_evict: too many tokens"); return CATCOC_E_TOO_LARGE; }
+  const int64_t capacity = static_cast<int64_t>(c->max_pages) * kPage, heads = static_cast<int64_t>(c->B) * c->Hk;
+  if (static_cast<int64_t>(c->recent) + c->sinks > c->keep) return bad("kv4_evict: the first and the last tokens are more than what is kept");
+  const int64_t most = std::min<int64_t>(c->keep, capacity);      // tokens that can stay
+  if (c->S < capacity || static_cast<int64_t>(c->out_pages) * kPage < most || c->S_out < most) return bad("kv4_evict: the weights or the new pages are too short");
+  if (unaligned(cache)) { set_error("kv4_evict: the cache must be 16-byte aligned"); return CATCOC_E_ALIGNMENT; }
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const bool in_place = out_table == block_table;
-  PickParams pick{weights, out_weights, kv_lens, kept, out_lens, B, Hk, S, S_out, keep, recent, sinks, static_cast<int>(capacity), status};
+  const PickParams pick{weights, out_weights, kv_lens, kept, out_lens, c->B, c->Hk, c->S, c->S_out, c->keep, c->recent, c->sinks, static_cast<int>(capacity), status};
   CATCOC_CUDA_OK(launch_overlapped(kv4_pick_kernel, dim3(static_cast<unsigned>(heads)), dim3(kPickThreads), 0, stream, pick));
-  MoveParams move{static_cast<uint8_t*>(cache), block_table, out_table, kept, out_lens, B, Hk, keep, max_pages, out_pages, pages, in_place, status};
+  const MoveParams move{static_cast<uint8_t*>(cache), block_table, out_table, kept, out_lens, c->B, c->Hk, c->keep, c->max_pages, c->out_pages, c->pages, in_place, status};
   const unsigned stretches = in_place ? 1u : static_cast<unsigned>(std::min<int64_t>(64, (most + 127) / 128));
   auto launch = [&](auto kernel) -> int {
     CATCOC_CUDA_OK(launch_overlapped(kernel, dim3(static_cast<unsigned>(heads), 2u, stretches), dim3(kMoveThreads), 0, stream, move));
     return CATCOC_OK;
   };
-  return D == 128 ? launch(kv4_move_kernel<128>) : launch(kv4_move_kernel<64>);
+  return c->D == 128 ? launch(kv4_move_kernel<128>) : launch(kv4_move_kernel<64>);
 }

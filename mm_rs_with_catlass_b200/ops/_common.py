@@ -213,6 +213,18 @@ def default_timeout_ns() -> int:
     return int(float(os.environ.get("CATCOC_TIMEOUT_MS", "10000")) * 1e6)
 
 
+_timeout = (None, 0)
+
+
+def timeout_ns() -> int:
+    """:func:`default_timeout_ns`, read anew on every call and worked out when it has changed."""
+    global _timeout
+    text = os.environ.get("CATCOC_TIMEOUT_MS", "10000")
+    if text != _timeout[0]:
+        _timeout = (text, default_timeout_ns())
+    return _timeout[1]
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 

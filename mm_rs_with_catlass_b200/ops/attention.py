@@ -27,6 +27,23 @@ from .. import _native as N
 from . import _common as cm
 
 
+def _shapes(q, k, v):
+    """(B, Hq, Hk, Sq, Sk, D) of the operands, checked."""
+    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        raise ValueError("flash_attention takes [B, H, S, D] tensors")
+    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("flash_attention takes fp16 / bf16 operands of one dtype")
+    b, hq, sq, d = q.shape
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise ValueError("k and v must be [B, Hk, Sk, D] with the batch and head dimension of q")
+    hk, sk = k.shape[1], k.shape[2]
+    if hq % hk:
+        raise ValueError("%d query heads do not divide over %d key / value heads" % (hq, hk))
+    if d not in (64, 128):
+        raise ValueError("head dimension %d: 64 and 128 are built" % d)
+    return b, hq, hk, sq, sk, d
+
+
 def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False,
                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None, window: Optional[int] = None,
                     sinks: int = 0) -> torch.Tensor:
@@ -43,28 +60,14 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
     ``p - j < window``, and the first ``sinks`` keys, ``j < sinks``, which stay visible to all. The work goes by what is
     visible: key blocks outside of a tile's windows are not read.
     """
+    if window is not None:
+        return _windowed(q, k, v, causal, scale, out, window, sinks)
+    if sinks:
+        raise ValueError("sinks belong to a window")
     dev = cm.require_cuda(q, k, v, out)
-    if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
-        raise ValueError("flash_attention takes [B, H, S, D] tensors")
-    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError("flash_attention takes fp16 / bf16 operands of one dtype")
-    b, hq, sq, d = q.shape
-    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
-        raise ValueError("k and v must be [B, Hk, Sk, D] with the batch and head dimension of q")
-    hk, sk = k.shape[1], k.shape[2]
-    if hq % hk:
-        raise ValueError("%d query heads do not divide over %d key / value heads" % (hq, hk))
-    if d not in (64, 128):
-        raise ValueError("head dimension %d: 64 and 128 are built" % d)
+    b, hq, hk, sq, sk, d = _shapes(q, k, v)
     if causal and sk < sq:
         raise ValueError("causal attention needs Sk >= Sq")
-    if window is not None:
-        if not causal:
-            raise ValueError("a window needs causal attention")
-        if window < 1 or sinks < 0:
-            raise ValueError("the window must be at least 1 and sinks not negative (got %d and %d)" % (window, sinks))
-    elif sinks:
-        raise ValueError("sinks belong to a window")
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
     if out is None:
         out = torch.empty_like(q)
@@ -76,15 +79,6 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
         raise ValueError("the softmax scale must be positive")
     with cm.guard(dev):
         lib, stream = N.lib(), C.c_void_p(cm.stream_of(dev))
-        if window is not None:
-            window, sinks = min(int(window), 1 << 30), min(int(sinks), 1 << 30)
-            need = int(lib.catcoc_window_route(b, hq, hk, sq, sk, d, window, sinks))
-            need = need if need >= 0 else -1 - need
-            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-            N.check(lib.catcoc_window_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ws.data_ptr() if need else None, b, hq, hk,
-                                                sq, sk, d, cm.out_fmt(q.dtype), window, sinks, float(scale), cm.local_status(dev).data_ptr(),
-                                                cm.default_timeout_ns(), stream))
-            return out
         tail = (b, hq, hk, sq, sk, d, cm.out_fmt(q.dtype), int(causal), float(scale), cm.local_status(dev).data_ptr(),
                 cm.default_timeout_ns(), stream)
         # few query rows per key / value head (decode steps): the keys are cut over the SMs instead of the queries; few tiles of
@@ -94,6 +88,53 @@ def flash_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal
         ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         N.check(kernel(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ws.data_ptr() if need else None, *tail))
     return out
+
+
+# What a windowed call has been found to be, by the layouts of its tensors and its numbers (never addresses): device, scratch, whether
+# operands are copied, the entry's numbers, the status block
+_windows: dict = {}
+
+
+def _windowed(q, k, v, causal, scale, out, window, sinks):
+    lay = cm.layout
+    key = (lay(q), lay(k), lay(v), lay(out), causal, scale, window, sinks)
+    plan = _windows.get(key)
+    if plan is None:
+        plan = _window_plan(q, k, v, causal, scale, out, window, sinks)
+        if len(_windows) >= 1024:
+            _windows.clear()
+        _windows[key] = plan
+    dev, need, copy, numbers, status = plan
+    if copy:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    if out is None:
+        out = torch.empty_like(q)
+    with cm.guard(dev):
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        N.check(N.lib().catcoc_window_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ws.data_ptr() if need else None, *numbers,
+                                                status, cm.timeout_ns(), cm.stream_of(dev)))
+    return out
+
+
+def _window_plan(q, k, v, causal, scale, out, window, sinks):
+    dev = cm.require_cuda(q, k, v, out)
+    b, hq, hk, sq, sk, d = _shapes(q, k, v)
+    if not causal:
+        raise ValueError("a window needs causal attention")
+    if sk < sq:
+        raise ValueError("causal attention needs Sk >= Sq")
+    if window < 1 or sinks < 0:
+        raise ValueError("the window must be at least 1 and sinks not negative (got %d and %d)" % (window, sinks))
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
+        raise ValueError("out must be a contiguous tensor shaped like q")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not scale > 0.0:
+        raise ValueError("the softmax scale must be positive")
+    window, sinks = min(int(window), 1 << 30), min(int(sinks), 1 << 30)
+    with cm.guard(dev):
+        need = int(N.lib().catcoc_window_route(b, hq, hk, sq, sk, d, window, sinks))
+    return (dev, need if need >= 0 else -1 - need, not all(x.is_contiguous() for x in (q, k, v)),
+            (b, hq, hk, sq, sk, d, cm.out_fmt(q.dtype), window, sinks, scale), cm.local_status(dev).data_ptr())
 
 
 def attention_reference(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, causal: bool = False,

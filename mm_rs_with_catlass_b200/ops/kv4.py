@@ -64,12 +64,58 @@ def _sequences(block_table: torch.Tensor, kv_lens: torch.Tensor) -> Tuple[int, i
     return batch, width
 
 
-def _aligned(x: torch.Tensor, dim: int) -> torch.Tensor:
-    """``x [T, H, dim]`` whose rows begin at 16-byte boundaries: itself, or a copy."""
+def _device_ints(t: Optional[torch.Tensor], name: str, batch: int) -> None:
+    if t is not None and (t.dtype != torch.int32 or tuple(t.shape) != (batch,) or not t.is_contiguous()):
+        raise ValueError("%s must be a contiguous int32 tensor [%d]" % (name, batch))
+
+
+def _weights(weights: torch.Tensor, batch: int, heads: int, tokens: int, what: str = "weights") -> None:
+    if weights.dtype != torch.float32 or weights.dim() != 3 or tuple(weights.shape[:2]) != (batch, heads) or not weights.is_contiguous():
+        raise ValueError("%s must be a contiguous fp32 tensor [%d, %d, tokens]" % (what, batch, heads))
+    if weights.shape[2] < tokens:
+        raise ValueError("%s must have room for %d tokens, as the block table has (got %d)" % (what, tokens, weights.shape[2]))
+
+
+# What a call has been found to be, by the layouts of its tensors and its numbers: checks are made and the numbers laid out once (a
+# decode step of one short sequence 20 -> 13 us a call). Addresses are no part of it.
+_plans: dict = {}
+
+
+class _Plan:
+    __slots__ = ("call", "at", "device", "status", "need", "copy")
+
+    def __init__(self, device, copy=(), need=0, **numbers):
+        self.call = N.Kv4Call(**numbers)
+        self.at = C.addressof(self.call)
+        self.device, self.status = device, cm.local_status(device).data_ptr()
+        self.need, self.copy = need, copy          # bytes of scratch, or shape of the results; which operands are copied first
+
+
+def _keep(key, plan: _Plan) -> _Plan:
+    if len(_plans) >= 1024:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _run(plan: _Plan, entry, *args) -> None:
+    device = plan.device
+    if cm.on_device(device):
+        N.check(entry(plan.at, *args, cm.stream_of(device)))
+    else:
+        with torch.cuda.device(device):
+            N.check(entry(plan.at, *args, cm.stream_of(device)))
+
+
+def _dense(x: torch.Tensor, copy: bool) -> torch.Tensor:
+    """``x``, or a copy of it where its rows do not begin at 16-byte boundaries (``copy``: by its strides)."""
+    return x.clone(memory_format=torch.contiguous_format) if copy or x.data_ptr() & 15 else x
+
+
+def _pitched(x: torch.Tensor) -> bool:
+    """Whether the rows of ``x [T, H, D]`` begin at 16-byte boundaries when ``x`` does."""
     s = x.stride()
-    if s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0 and x.data_ptr() % 16 == 0:
-        return x
-    return x.clone(memory_format=torch.contiguous_format)
+    return s[2] == 1 and s[0] % 8 == 0 and s[1] % 8 == 0
 
 
 def kv4_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, *,
@@ -84,27 +130,32 @@ def kv4_append(cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_tabl
     A group of 64 channels gets ``s = bf16((max - min) / 15)``, ``z = bf16(min)`` and the codes ``rint((x - z) / s)``, at most
     15, taken with ``1 / s`` in fp32; it stands for ``s * code + z``.
     """
-    dev = cm.require_cuda(cache, k, v, block_table, kv_lens, ends)
-    pages, heads, d = _cache_dims(cache)
-    batch, width = _sequences(block_table, kv_lens)
-    if k.dim() != 3 or k.shape != v.shape or k.shape[1] != heads or k.shape[2] != d:
-        raise ValueError("k and v must be [T, %d, %d] for this cache, got %s and %s" % (heads, d, tuple(k.shape), tuple(v.shape)))
-    if k.dtype not in _FMT or v.dtype != k.dtype:
-        raise TypeError("kv4_append takes fp16 / bf16 keys and values of one dtype")
-    tokens = k.shape[0]
-    if ends is None:
-        if tokens % batch:
-            raise ValueError("%d tokens do not divide over %d sequences; give ends" % (tokens, batch))
-    elif ends.dtype != torch.int32 or tuple(ends.shape) != (batch,) or not ends.is_contiguous():
-        raise ValueError("ends must be a contiguous int32 tensor [%d]" % batch)
-    if not tokens:
+    lay = cm.layout
+    key = (0, lay(cache), lay(k), lay(v), lay(block_table), lay(kv_lens), lay(ends))
+    plan = _plans.get(key)
+    if plan is None:
+        dev = cm.require_cuda(cache, k, v, block_table, kv_lens, ends)
+        pages, heads, d = _cache_dims(cache)
+        batch, width = _sequences(block_table, kv_lens)
+        if k.dim() != 3 or k.shape != v.shape or k.shape[1] != heads or k.shape[2] != d:
+            raise ValueError("k and v must be [T, %d, %d] for this cache, got %s and %s" % (heads, d, tuple(k.shape), tuple(v.shape)))
+        if k.dtype not in _FMT or v.dtype != k.dtype:
+            raise TypeError("kv4_append takes fp16 / bf16 keys and values of one dtype")
+        if ends is None and k.shape[0] % batch:
+            raise ValueError("%d tokens do not divide over %d sequences; give ends" % (k.shape[0], batch))
+        _device_ints(ends, "ends", batch)
+        copy = (not _pitched(k), not _pitched(v))
+        rows = (heads * d, d)
+        (kt, kh), (vt, vh) = (rows if c else x.stride()[:2] for x, c in ((k, copy[0]), (v, copy[1])))
+        plan = _keep(key, _Plan(dev, copy, B=batch, Hk=heads, D=d, pages=pages, max_pages=width, fmt=_FMT[k.dtype], T=k.shape[0],
+                                k_token=kt, k_head=kh, v_token=vt, v_head=vh))
+    if not plan.call.T:
         return cache
-    k, v = _aligned(k, d), _aligned(v, d)
-    with cm.guard(dev):
-        N.check(N.lib().catcoc_kv4_append(cache.data_ptr(), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
-                                          block_table.data_ptr(), kv_lens.data_ptr(), ends.data_ptr() if ends is not None else None, tokens,
-                                          batch, heads, d, pages, width, _FMT[k.dtype], cm.local_status(dev).data_ptr(),
-                                          C.c_void_p(cm.stream_of(dev))))
+    if plan.copy[0] or plan.copy[1] or (k.data_ptr() | v.data_ptr()) & 15:
+        # (a base between two boundaries: the rows of the copy are dense, which is another call)
+        return kv4_append(cache, _dense(k, plan.copy[0]), _dense(v, plan.copy[1]), block_table, kv_lens, ends=ends)
+    _run(plan, N.lib().catcoc_kv4_append, cache.data_ptr(), k.data_ptr(), v.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(),
+         ends.data_ptr() if ends is not None else None, plan.status)
     return cache
 
 
@@ -113,29 +164,25 @@ def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tens
     """``(k, v)``, each ``[B, Hk, count, D]`` in fp16 / bf16: the values of the cache's tokens at the positions ``start[b]`` to
     ``start[b] + count - 1`` (``start`` ``[B]``, int32; from the beginning without it; ``count``: as many as the table's
     row can hold), zero where a sequence has no token."""
-    dev = cm.require_cuda(cache, block_table, kv_lens, start)
-    pages, heads, d = _cache_dims(cache)
-    batch, width = _sequences(block_table, kv_lens)
-    if dtype not in _FMT:
-        raise TypeError("kv4_read gives fp16 / bf16")
-    if start is not None and (start.dtype != torch.int32 or tuple(start.shape) != (batch,) or not start.is_contiguous()):
-        raise ValueError("start must be a contiguous int32 tensor [%d]" % batch)
-    count = width * PAGE if count is None else int(count)
-    if count < 1:
-        raise ValueError("count must be positive")
-    k, v = (torch.empty((batch, heads, count, d), dtype=dtype, device=dev) for _ in range(2))
-    with cm.guard(dev):
-        N.check(N.lib().catcoc_kv4_read(cache.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), start.data_ptr() if start is not None else None,
-                                        k.data_ptr(), v.data_ptr(), batch, heads, d, pages, width, count, _FMT[dtype],
-                                        cm.local_status(dev).data_ptr(), C.c_void_p(cm.stream_of(dev))))
+    lay = cm.layout
+    key = (1, lay(cache), lay(block_table), lay(kv_lens), lay(start), count, dtype)
+    plan = _plans.get(key)
+    if plan is None:
+        dev = cm.require_cuda(cache, block_table, kv_lens, start)
+        pages, heads, d = _cache_dims(cache)
+        batch, width = _sequences(block_table, kv_lens)
+        if dtype not in _FMT:
+            raise TypeError("kv4_read gives fp16 / bf16")
+        _device_ints(start, "start", batch)
+        n = width * PAGE if count is None else int(count)
+        if n < 1:
+            raise ValueError("count must be positive")
+        plan = _keep(key, _Plan(dev, B=batch, Hk=heads, D=d, pages=pages, max_pages=width, fmt=_FMT[dtype], count=n))
+        plan.need = (batch, heads, n, d)
+    k, v = torch.empty(plan.need, dtype=dtype, device=plan.device), torch.empty(plan.need, dtype=dtype, device=plan.device)
+    _run(plan, N.lib().catcoc_kv4_read, cache.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), start.data_ptr() if start is not None else None,
+         k.data_ptr(), v.data_ptr(), plan.status)
     return k, v
-
-
-def _weights(weights: torch.Tensor, batch: int, heads: int, tokens: int, what: str = "weights") -> None:
-    if weights.dtype != torch.float32 or weights.dim() != 3 or tuple(weights.shape[:2]) != (batch, heads) or not weights.is_contiguous():
-        raise ValueError("%s must be a contiguous fp32 tensor [%d, %d, tokens]" % (what, batch, heads))
-    if weights.shape[2] < tokens:
-        raise ValueError("%s must have room for %d tokens, as the block table has (got %d)" % (what, tokens, weights.shape[2]))
 
 
 def kv4_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, *, q_len: int = 1,
@@ -150,6 +197,22 @@ def kv4_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, 
     are added to it, position by position: what :func:`kv4_evict` goes by. Returns ``[T, Hq, D]``; a token that sees nothing
     gives zeros.
     """
+    lay = cm.layout
+    key = (2, lay(q), lay(cache), lay(block_table), lay(kv_lens), lay(weights), lay(out), q_len, window, sinks, scale)
+    plan = _plans.get(key)
+    if plan is None:
+        plan = _keep(key, _decode_plan(q, cache, block_table, kv_lens, q_len, window, sinks, weights, scale, out))
+    q = _dense(q, plan.copy)
+    if out is None:
+        out = torch.empty_like(q)
+    # scratch of the caching allocator: calls on several streams never share one
+    ws = torch.empty(plan.need, dtype=torch.uint8, device=plan.device)
+    _run(plan, N.lib().catcoc_kv4_decode, q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), out.data_ptr(),
+         weights.data_ptr() if weights is not None else None, ws.data_ptr(), plan.status, cm.timeout_ns())
+    return out
+
+
+def _decode_plan(q, cache, block_table, kv_lens, q_len, window, sinks, weights, scale, out) -> _Plan:
     dev = cm.require_cuda(q, cache, block_table, kv_lens, weights, out)
     pages, heads, d = _cache_dims(cache)
     batch, width = _sequences(block_table, kv_lens)
@@ -176,25 +239,15 @@ def kv4_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, 
         raise ValueError("the softmax scale must be positive")
     if weights is not None:
         _weights(weights, batch, heads, width * PAGE)
-    if not q.is_contiguous() or q.data_ptr() % 16:
-        q = q.clone(memory_format=torch.contiguous_format)
-    if out is None:
-        out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
         raise ValueError("out must be a contiguous tensor shaped like q")
-    window, sinks = min(int(window), 1 << 30), min(int(sinks), 1 << 30)
-    lib = N.lib()
+    plan = _Plan(dev, not q.is_contiguous(), B=batch, Hk=heads, D=d, pages=pages, max_pages=width, fmt=_FMT[q.dtype], Hq=hq, q_len=q_len,
+                 window=min(int(window), 1 << 30), sinks=min(int(sinks), 1 << 30), scale=float(scale), S=weights.shape[2] if weights is not None else 0)
     with cm.guard(dev):
-        need = int(lib.catcoc_kv4_decode_workspace_bytes(batch, q_len, hq, heads, d, width, window, sinks, int(weights is not None)))
-        if need < 0:
-            raise ValueError("kv4_decode: %d sequences of %d pages with %d rows a head are more than the kernel takes" % (batch, width, hq // heads * q_len))
-        # scratch of the caching allocator: calls on several streams never share one
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        N.check(lib.catcoc_kv4_decode(q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), out.data_ptr(),
-                                      weights.data_ptr() if weights is not None else None, weights.shape[2] if weights is not None else 0,
-                                      ws.data_ptr(), batch, q_len, hq, heads, d, pages, width, window, sinks, _FMT[q.dtype], float(scale),
-                                      cm.local_status(dev).data_ptr(), cm.default_timeout_ns(), C.c_void_p(cm.stream_of(dev))))
-    return out
+        plan.need = int(N.lib().catcoc_kv4_decode_workspace_bytes(plan.at, int(weights is not None)))
+    if plan.need < 0:
+        raise ValueError("kv4_decode: %d sequences of %d pages with %d rows a head are more than the kernel takes" % (batch, width, hq // heads * q_len))
+    return plan
 
 
 def kv4_evict(cache: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, keep: int, *, recent: int = 0,
@@ -209,31 +262,33 @@ def kv4_evict(cache: torch.Tensor, weights: torch.Tensor, block_table: torch.Ten
     int32 ``[B, Hk, keep]``, the positions that the tokens had (-1 behind the last), and the new lengths
     ``min(kv_lens, keep)`` as a new int32 tensor. ``block_table`` and ``kv_lens`` are not changed.
     """
-    dev = cm.require_cuda(cache, weights, block_table, kv_lens, out_table, out_weights)
-    pages, heads, d = _cache_dims(cache)
-    batch, width = _sequences(block_table, kv_lens)
-    keep, recent, sinks = int(keep), int(recent), int(sinks)
-    if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
-        raise ValueError("keep=%d must be positive and hold the %d first and %d last tokens" % (keep, sinks, recent))
-    _weights(weights, batch, heads, width * PAGE)
-    most = min(keep, width * PAGE)
-    if out_table is None:
-        out_table = block_table
-    elif out_table.dtype != torch.int32 or out_table.dim() != 2 or out_table.shape[0] != batch or not out_table.is_contiguous():
-        raise ValueError("out_table must be a contiguous int32 tensor [%d, max_pages]" % batch)
-    elif out_table.shape[1] * PAGE < most:
-        raise ValueError("out_table must name pages for %d tokens" % most)
-    if out_weights is None:
-        out_weights = weights
-    else:
-        _weights(out_weights, batch, heads, most, "out_weights")
-    kept = torch.empty((batch, heads, keep), dtype=torch.int32, device=dev)
-    lens = torch.empty(batch, dtype=torch.int32, device=dev)
-    with cm.guard(dev):
-        N.check(N.lib().catcoc_kv4_evict(cache.data_ptr(), weights.data_ptr(), out_weights.data_ptr(), block_table.data_ptr(), out_table.data_ptr(),
-                                         kv_lens.data_ptr(), kept.data_ptr(), lens.data_ptr(), batch, heads, d, pages, width, out_table.shape[1],
-                                         weights.shape[2], out_weights.shape[2], keep, recent, sinks, cm.local_status(dev).data_ptr(),
-                                         C.c_void_p(cm.stream_of(dev))))
+    lay = cm.layout
+    key = (3, lay(cache), lay(weights), lay(block_table), lay(kv_lens), lay(out_table), lay(out_weights), keep, recent, sinks)
+    plan = _plans.get(key)
+    if plan is None:
+        dev = cm.require_cuda(cache, weights, block_table, kv_lens, out_table, out_weights)
+        pages, heads, d = _cache_dims(cache)
+        batch, width = _sequences(block_table, kv_lens)
+        keep, recent, sinks = int(keep), int(recent), int(sinks)
+        if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
+            raise ValueError("keep=%d must be positive and hold the %d first and %d last tokens" % (keep, sinks, recent))
+        _weights(weights, batch, heads, width * PAGE)
+        most = min(keep, width * PAGE)
+        if out_table is not None:
+            if out_table.dtype != torch.int32 or out_table.dim() != 2 or out_table.shape[0] != batch or not out_table.is_contiguous():
+                raise ValueError("out_table must be a contiguous int32 tensor [%d, max_pages]" % batch)
+            if out_table.shape[1] * PAGE < most:
+                raise ValueError("out_table must name pages for %d tokens" % most)
+        if out_weights is not None:
+            _weights(out_weights, batch, heads, most, "out_weights")
+        plan = _keep(key, _Plan(dev, B=batch, Hk=heads, D=d, pages=pages, max_pages=width, S=weights.shape[2], keep=keep, recent=recent, sinks=sinks,
+                                S_out=(weights if out_weights is None else out_weights).shape[2],
+                                out_pages=(block_table if out_table is None else out_table).shape[1]))
+        plan.need = (batch, heads, keep)
+    kept, lens = torch.empty(plan.need, dtype=torch.int32, device=plan.device), torch.empty_like(kv_lens)
+    _run(plan, N.lib().catcoc_kv4_evict, cache.data_ptr(), weights.data_ptr(), (weights if out_weights is None else out_weights).data_ptr(),
+         block_table.data_ptr(), (block_table if out_table is None else out_table).data_ptr(), kv_lens.data_ptr(), kept.data_ptr(), lens.data_ptr(),
+         plan.status)
     return kept, lens
 
 

@@ -1,4 +1,5 @@
 """The 4-bit cache without a GPU: the goldens against the formulas, the layout of a block, and everything the functions refuse."""
+import ctypes
 import math
 
 import pytest
@@ -165,21 +166,38 @@ def test_refusals(monkeypatch):
 def test_the_library_refuses_too():
     """The C entries check what they are given before any launch (no GPU here: a call that passed would fail otherwise)."""
     lib, one = N.lib(), 16
-    append = lambda **k: lib.catcoc_kv4_append(*[{**dict(cache=one, k=one, kt=64, kh=64, v=one, vt=64, vh=64, table=one, lens=one, ends=None, T=2,
-                                                        B=2, Hk=1, D=64, pages=1, width=1, fmt=N.FMT_BF16, status=one, stream=None), **k}[n]
-                                                 for n in "cache k kt kh v vt vh table lens ends T B Hk D pages width fmt status stream".split()])
-    assert append(T=0) == N.E_BAD_ARG and append(T=3) == N.E_BAD_ARG and append(lens=None) == N.E_BAD_ARG
-    assert append(D=96) == N.E_UNSUPPORTED and append(fmt=N.FMT_F32) == N.E_UNSUPPORTED
-    assert append(kt=65) == N.E_ALIGNMENT and append(v=18) == N.E_ALIGNMENT and append(width=1 << 27) == N.E_TOO_LARGE
-    space = lib.catcoc_kv4_decode_workspace_bytes
-    assert space(2, 1, 3, 2, 64, 4, 0, 0, 0) == -1 and space(2, 65, 4, 2, 64, 4, 0, 0, 0) == -1 and space(2, 1, 4, 2, 96, 4, 0, 0, 0) == -1
-    assert space(4097, 1, 4, 2, 64, 4, 0, 0, 0) == -1 and space(2, 64, 128, 1, 64, 4, 0, 0, 0) == -1 and space(1, 1, 1, 1, 64, 1 << 19, 0, 0, 0) == -1
-    evict = lambda **k: lib.catcoc_kv4_evict(*[{**dict(cache=one, w=one, ow=one, table=one, otable=one, lens=one, kept=one, olens=one, B=1, Hk=1, D=64,
-                                                      pages=4, width=2, owidth=2, S=128, So=128, keep=4, recent=2, sinks=2, status=one, stream=None), **k}[n]
-                                               for n in "cache w ow table otable lens kept olens B Hk D pages width owidth S So keep recent sinks status stream".split()])
-    assert evict(sinks=3) == N.E_BAD_ARG and evict(S=127) == N.E_BAD_ARG and evict(keep=0) == N.E_BAD_ARG and evict(kept=None) == N.E_BAD_ARG
-    assert evict(keep=100, owidth=1) == N.E_BAD_ARG and evict(keep=100, So=99) == N.E_BAD_ARG and evict(D=32) == N.E_UNSUPPORTED and evict(cache=8) == N.E_ALIGNMENT
-    read = lambda **k: lib.catcoc_kv4_read(*[{**dict(cache=one, table=one, lens=one, start=None, k=one, v=one, B=1, Hk=1, D=64, pages=1, width=1, count=1,
-                                                    fmt=N.FMT_F16, status=one, stream=None), **k}[n]
-                                             for n in "cache table lens start k v B Hk D pages width count fmt status stream".split()])
-    assert read(count=0) == N.E_BAD_ARG and read(D=65) == N.E_UNSUPPORTED and read(k=8) == N.E_ALIGNMENT and read(count=1 << 22) == N.E_TOO_LARGE
+
+    def call(**changes):
+        numbers = dict(B=2, Hk=1, D=64, pages=4, max_pages=2, fmt=N.FMT_BF16, T=2, count=1, keep=4, recent=2, sinks=2, out_pages=2, S=128, S_out=128,
+                       Hq=4, q_len=1, window=0, scale=1.0, k_token=64, k_head=64, v_token=64, v_head=64)
+        return N.Kv4Call(**{**numbers, **changes})
+
+    def run(entry, pointers, null=None, odd=None, **changes):
+        c = call(**changes)
+        args = [None if i == null else 8 if i == odd else one for i in range(pointers)]
+        tail = (0, None) if entry is lib.catcoc_kv4_decode else (None,)
+        return entry(ctypes.addressof(c), *args, *tail)
+
+    append, read, evict, decode = lib.catcoc_kv4_append, lib.catcoc_kv4_read, lib.catcoc_kv4_evict, lib.catcoc_kv4_decode
+
+    def space(**changes):
+        c = call(**changes)
+        return lib.catcoc_kv4_decode_workspace_bytes(ctypes.addressof(c), 1)
+    for entry, pointers in ((append, 7), (read, 7), (evict, 9), (decode, 8)):
+        for bad in (dict(B=0), dict(Hk=0), dict(pages=0), dict(max_pages=0)):
+            assert run(entry, pointers, **bad) == N.E_BAD_ARG
+        assert run(entry, pointers, null=0) == N.E_BAD_ARG and run(entry, pointers, null=pointers - 1) == N.E_BAD_ARG
+        assert entry(None, *[one] * pointers, *((0, None) if entry is decode else (None,))) == N.E_BAD_ARG
+    assert run(append, 7, T=0) == N.E_BAD_ARG and run(append, 7, null=5, T=3) == N.E_BAD_ARG and run(append, 7, null=4) == N.E_BAD_ARG
+    assert run(append, 7, D=96) == N.E_UNSUPPORTED and run(append, 7, fmt=N.FMT_F32) == N.E_UNSUPPORTED
+    assert run(append, 7, k_token=65) == N.E_ALIGNMENT and run(append, 7, odd=2) == N.E_ALIGNMENT and run(append, 7, max_pages=1 << 27) == N.E_TOO_LARGE
+    assert run(read, 7, count=0) == N.E_BAD_ARG and run(read, 7, D=65) == N.E_UNSUPPORTED and run(read, 7, odd=4) == N.E_ALIGNMENT
+    assert run(read, 7, count=1 << 22) == N.E_TOO_LARGE
+    assert run(evict, 9, sinks=3) == N.E_BAD_ARG and run(evict, 9, S=127) == N.E_BAD_ARG and run(evict, 9, keep=0) == N.E_BAD_ARG
+    assert run(evict, 9, keep=100, out_pages=1) == N.E_BAD_ARG and run(evict, 9, keep=100, S_out=99) == N.E_BAD_ARG
+    assert run(evict, 9, D=32) == N.E_UNSUPPORTED and run(evict, 9, odd=0) == N.E_ALIGNMENT
+    for bad in (dict(Hq=3, Hk=2), dict(q_len=65), dict(q_len=0), dict(D=96), dict(B=4097), dict(q_len=64, Hq=128), dict(max_pages=1 << 19), dict(window=-1),
+                dict(sinks=-1)):
+        assert space(**bad) == -1 and run(decode, 8, **bad) == N.E_BAD_ARG
+    assert run(decode, 8, scale=0.0) == N.E_UNSUPPORTED and run(decode, 8, scale=float("nan")) == N.E_UNSUPPORTED
+    assert run(decode, 8, S=127) == N.E_BAD_ARG and run(decode, 8, odd=0) == N.E_ALIGNMENT and space() > 0
