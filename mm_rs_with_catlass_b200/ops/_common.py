@@ -174,8 +174,21 @@ def tkey(t: Optional[torch.Tensor]):
     return (t.data_ptr(), t.shape, t.stride(), t.dtype)
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)   # (a tensor on a device: CUDA is up)
+
+
 def on_device(device: torch.device) -> bool:
-    return torch.cuda.current_device() == (device.index if device.index is not None else 0)
+    return _current_device() == (device.index if device.index is not None else 0)
+
+
+def like(shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    """What :func:`fresh` makes tensors like: a view of one element, to be kept."""
+    return torch.empty(1, dtype=dtype, device=device).expand(shape)
+
+
+def fresh(template: torch.Tensor) -> torch.Tensor:
+    """An uninitialised dense tensor of the template's shape: a third of what ``torch.empty`` takes to read its arguments."""
+    return torch.empty_like(template, memory_format=torch.contiguous_format)
 
 
 _NO_GUARD = contextlib.nullcontext()

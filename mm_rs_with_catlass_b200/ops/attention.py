@@ -104,15 +104,15 @@ def _windowed(q, k, v, causal, scale, out, window, sinks):
         if len(_windows) >= 1024:
             _windows.clear()
         _windows[key] = plan
-    dev, need, copy, numbers, status = plan
+    dev, scratch, copy, numbers, status = plan
     if copy:
         q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
     if out is None:
         out = torch.empty_like(q)
     with cm.guard(dev):
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        N.check(N.lib().catcoc_window_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ws.data_ptr() if need else None, *numbers,
-                                                status, cm.timeout_ns(), cm.stream_of(dev)))
+        ws = cm.fresh(scratch) if scratch is not None else None
+        N.check(N.lib().catcoc_window_attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), ws.data_ptr() if ws is not None else None,
+                                                *numbers, status, cm.timeout_ns(), cm.stream_of(dev)))
     return out
 
 
@@ -133,7 +133,8 @@ def _window_plan(q, k, v, causal, scale, out, window, sinks):
     window, sinks = min(int(window), 1 << 30), min(int(sinks), 1 << 30)
     with cm.guard(dev):
         need = int(N.lib().catcoc_window_route(b, hq, hk, sq, sk, d, window, sinks))
-    return (dev, need if need >= 0 else -1 - need, not all(x.is_contiguous() for x in (q, k, v)),
+    need = need if need >= 0 else -1 - need
+    return (dev, cm.like((need,), torch.uint8, dev) if need else None, not all(x.is_contiguous() for x in (q, k, v)),
             (b, hq, hk, sq, sk, d, cm.out_fmt(q.dtype), window, sinks, scale), cm.local_status(dev).data_ptr())
 
 

@@ -82,13 +82,13 @@ _plans: dict = {}
 
 
 class _Plan:
-    __slots__ = ("call", "at", "device", "status", "need", "copy")
+    __slots__ = ("call", "at", "device", "status", "fresh", "copy")
 
-    def __init__(self, device, copy=(), need=0, **numbers):
+    def __init__(self, device, copy=(), **numbers):
         self.call = N.Kv4Call(**numbers)
         self.at = C.addressof(self.call)
         self.device, self.status = device, cm.local_status(device).data_ptr()
-        self.need, self.copy = need, copy          # bytes of scratch, or shape of the results; which operands are copied first
+        self.copy, self.fresh = copy, None         # which operands are copied first; what results or scratch are made like
 
 
 def _keep(key, plan: _Plan) -> _Plan:
@@ -178,8 +178,8 @@ def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tens
         if n < 1:
             raise ValueError("count must be positive")
         plan = _keep(key, _Plan(dev, B=batch, Hk=heads, D=d, pages=pages, max_pages=width, fmt=_FMT[dtype], count=n))
-        plan.need = (batch, heads, n, d)
-    k, v = torch.empty(plan.need, dtype=dtype, device=plan.device), torch.empty(plan.need, dtype=dtype, device=plan.device)
+        plan.fresh = cm.like((batch, heads, n, d), dtype, dev)
+    k, v = cm.fresh(plan.fresh), cm.fresh(plan.fresh)
     _run(plan, N.lib().catcoc_kv4_read, cache.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), start.data_ptr() if start is not None else None,
          k.data_ptr(), v.data_ptr(), plan.status)
     return k, v
@@ -206,7 +206,7 @@ def kv4_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, 
     if out is None:
         out = torch.empty_like(q)
     # scratch of the caching allocator: calls on several streams never share one
-    ws = torch.empty(plan.need, dtype=torch.uint8, device=plan.device)
+    ws = cm.fresh(plan.fresh)
     _run(plan, N.lib().catcoc_kv4_decode, q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), out.data_ptr(),
          weights.data_ptr() if weights is not None else None, ws.data_ptr(), plan.status, cm.timeout_ns())
     return out
@@ -244,9 +244,10 @@ def _decode_plan(q, cache, block_table, kv_lens, q_len, window, sinks, weights, 
     plan = _Plan(dev, not q.is_contiguous(), B=batch, Hk=heads, D=d, pages=pages, max_pages=width, fmt=_FMT[q.dtype], Hq=hq, q_len=q_len,
                  window=min(int(window), 1 << 30), sinks=min(int(sinks), 1 << 30), scale=float(scale), S=weights.shape[2] if weights is not None else 0)
     with cm.guard(dev):
-        plan.need = int(N.lib().catcoc_kv4_decode_workspace_bytes(plan.at, int(weights is not None)))
-    if plan.need < 0:
+        need = int(N.lib().catcoc_kv4_decode_workspace_bytes(plan.at, int(weights is not None)))
+    if need < 0:
         raise ValueError("kv4_decode: %d sequences of %d pages with %d rows a head are more than the kernel takes" % (batch, width, hq // heads * q_len))
+    plan.fresh = cm.like((need,), torch.uint8, dev)
     return plan
 
 
@@ -284,8 +285,8 @@ def kv4_evict(cache: torch.Tensor, weights: torch.Tensor, block_table: torch.Ten
         plan = _keep(key, _Plan(dev, B=batch, Hk=heads, D=d, pages=pages, max_pages=width, S=weights.shape[2], keep=keep, recent=recent, sinks=sinks,
                                 S_out=(weights if out_weights is None else out_weights).shape[2],
                                 out_pages=(block_table if out_table is None else out_table).shape[1]))
-        plan.need = (batch, heads, keep)
-    kept, lens = torch.empty(plan.need, dtype=torch.int32, device=plan.device), torch.empty_like(kv_lens)
+        plan.fresh = cm.like((batch, heads, keep), torch.int32, dev)
+    kept, lens = cm.fresh(plan.fresh), torch.empty_like(kv_lens)
     _run(plan, N.lib().catcoc_kv4_evict, cache.data_ptr(), weights.data_ptr(), (weights if out_weights is None else out_weights).data_ptr(),
          block_table.data_ptr(), (block_table if out_table is None else out_table).data_ptr(), kv_lens.data_ptr(), kept.data_ptr(), lens.data_ptr(),
          plan.status)
