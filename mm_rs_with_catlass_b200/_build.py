@@ -50,6 +50,7 @@ SOURCES = [
     "kernels/small_allreduce.cu",
     "kernels/flash_attn.cu",
     "kernels/flash_decode.cu",
+    "kernels/window_attn.cu",
     "kernels/mla_decode.cu",
     "kernels/mla_rows.cu",
     "kernels/kv4_cache.cu",

@@ -67,7 +67,6 @@ struct AttnParams {
   float* part_o;                  // keys cut into slices: [slice][B * Hq * Sq][D] unnormalised pieces
   float* part_ml;                 // [slice][B * Hq * Sq][2]
   int per;                        // key blocks of a slice
-  int window, sinks;              // WINDOW: position i sees of the keys up to its own the last `window` and the first `sinks`
 };
 
 struct Bars {
@@ -85,9 +84,8 @@ CATCOC_DEVICE void fail(const AttnParams& p, uint32_t what, uint32_t a, uint32_t
 
 // D: head dimension; FMT: operand and output dtype (compile time: the softmax loop packs 64 pairs per row and block);
 // CUT: a CTA takes the key blocks of slice blockIdx.y only and leaves a piece; LATE: a block's softmax waits for the product with V of
-// the block before where it needs it, to rescale O or to write P, else ahead of its exponentials (D = 64, see attn_plan); WINDOW: a
-// causal call in which a tile walks the blocks of the first keys (sinks) and of its rows' windows alone
-template <int D, int FMT, bool CUT, bool LATE, bool WINDOW>
+// the block before where it needs it, to rescale O or to write P, else ahead of its exponentials (D = 64, see attn_plan)
+template <int D, int FMT, bool CUT, bool LATE>
 __global__ void __launch_bounds__(kThreads, 1) flash_attn_kernel(const __grid_constant__ AttnParams p) {
   constexpr int kDB = D / 64;                    // 128-byte blocks along the head dimension
   constexpr int kQBytes = kDB * kBlockBytes;     // one Q tile
@@ -132,31 +130,6 @@ __global__ void __launch_bounds__(kThreads, 1) flash_attn_kernel(const __grid_co
     const int kv_end = p.causal ? min(p.Sk, tile_hi(t) + 1 + shift) : p.Sk;
     nblk[t] = (kv_end + kBKV - 1) / kBKV;
   }
-  // With a window the CTA's list of blocks is that of the sinks, then from the first block that some row's window reaches. Both tiles walk it
-  // from its start; a block in front of tile 1's windows (`skip`) stands behind the blocks of both, ahead of tile 1's last one, and is left out
-  // by tile 1, so that both walk as many blocks as they see and start in step. 1 x 32 / 8 heads x 8192, window 1024: 10 blocks a tile where 11 would be walked.
-  int sink_blocks = 0, first = 0, shared = 0;
-  bool skip = false;
-  if constexpr (WINDOW) {
-    auto first_of = [&](int t) { return max(0, tile_lo(t) + shift - p.window + 1) / kBKV; };
-    const bool second = q0 + kBQ < p.Sq;                              // (else no row of tile 1 exists)
-    if (!second) nblk[1] = nblk[0];
-    const int first1 = first_of(second ? 1 : 0), want = (p.sinks + kBKV - 1) / kBKV, end0 = nblk[0];
-    first = min(first_of(0), first1);
-    sink_blocks = min(want, first);
-    skip = !CUT && first1 == first + 1 && nblk[1] == end0 + 1 && first >= want;
-    shared = sink_blocks + end0 - first - 1;                          // with `skip`: blocks of both
-#pragma unroll
-    for (int t = 0; t < kTiles; ++t) nblk[t] += sink_blocks - first - (skip && t == 1 ? 1 : 0);
-  }
-  // key block of an item of the list, and the item that a tile takes as its j-th
-  auto block_of = [&](int item) {
-    if constexpr (!WINDOW) return item;
-    if (item < sink_blocks) return item;
-    if (!skip) return first + item - sink_blocks;
-    return item == shared ? first : first + item - sink_blocks + (item < shared ? 1 : 0);
-  };
-  auto item_of = [&](int t, int j) { return WINDOW && skip && t == 1 && j == shared ? j + 1 : j; };
   // (a slice that some tile sees nothing of is a masked block there: a maximum of -inf, a sum of zero)
   const int j0 = CUT ? static_cast<int>(blockIdx.y) * p.per : 0;
   if constexpr (CUT) {
@@ -164,7 +137,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_attn_kernel(const __grid_co
     for (int t = 0; t < kTiles; ++t) nblk[t] = max(1, min(p.per, nblk[t] - j0));
   }
   nblk[1] = max(nblk[0], nblk[1]);
-  const int nmax = nblk[1] + (WINDOW && skip ? 1 : 0);             // items of the list
+  const int nmax = nblk[1];
 
   if (threadIdx.x == 0) {
     ptx::mbar_init(&bars->q_full, 1);
@@ -211,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_attn_kernel(const __grid_co
         ptx::mbar_expect_tx(&bars->kv_full[slot], kSlotBytes);
         const CUtensorMap* tm = (item & 1) ? &p.tm_v : &p.tm_k;
         for (int d = 0; d < kDB; ++d)
-          ptx::tma_load_3d(skv + slot * kSlotBytes + d * kBlockBytes, tm, &bars->kv_full[slot], d * 64, block_of(j0 + (item >> 1)) * kBKV, bhk);
+          ptx::tma_load_3d(skv + slot * kSlotBytes + d * kBlockBytes, tm, &bars->kv_full[slot], d * 64, (j0 + (item >> 1)) * kBKV, bhk);
       }
       __syncwarp();
     }
@@ -227,18 +200,17 @@ __global__ void __launch_bounds__(kThreads, 1) flash_attn_kernel(const __grid_co
     auto wait_item = [&](int item) {
       return ptx::mbar_wait(&bars->kv_full[item % kSlots], static_cast<uint32_t>(item / kSlots) & 1u, p.timeout_ns, abort_flag);
     };
-    // (one warp for both tiles has waited for tile 0's block when it comes to tile 1, and hands it back when tile 1 has used it too)
-    auto first_use = [&](int t, int j) { return kOneS || t == 0 || j >= nblk[0] || item_of(1, j) != j; };
-    auto last_use = [&](int t, int j) { return kOneS || t == 1 || (WINDOW && skip && j == shared); };
+    // (one warp for both tiles has waited for tile 0's block when it comes to tile 1)
+    auto first_use = [&](int t, int j) { return kOneS || t == 0 || j >= nblk[0]; };
     // S_t[128, 128 keys] = Q_t[128, D] K^T of block j, behind the softmax's read of what is in the buffer: both operands
     // K-major (D contiguous), 16 elements of D per MMA
     auto scores = [&](int t, int j) {
-      if (first_use(t, j) && !wait_item(2 * item_of(t, j))) return false;
+      if (first_use(t, j) && !wait_item(2 * j)) return false;
       const int before = !kOneS || t == 0 || j >= nblk[0] ? j - 1 : j;             // the block and the tile that were there
       const int tile = !kOneS ? t : (t == 1 && j < nblk[0] ? 0 : 1);
       if (before >= 0 && !ptx::mbar_wait(&bars->s_free[tile], static_cast<uint32_t>(before & 1), p.timeout_ns, abort_flag)) return false;
       ptx::tcgen05_fence_after();
-      const int slot = (2 * item_of(t, j)) % kSlots;
+      const int slot = (2 * j) % kSlots;
       if (ptx::elect_one()) {
         const uint32_t ql = q_lo + static_cast<uint32_t>(t * (kQBytes >> 4)), kl = k_lo + static_cast<uint32_t>(slot * (kSlotBytes >> 4));
 #pragma unroll
@@ -247,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_attn_kernel(const __grid_co
           ptx::umma_f16(tmem + (kOneS ? 0 : t * 128), ptx::desc_of(ql + off, q_hi), ptx::desc_of(kl + off, k_hi), p.idesc_qk, kk != 0 ? 1u : 0u);
         }
         ptx::tcgen05_commit(&bars->s_full[t]);
-        if (last_use(t, j)) ptx::tcgen05_commit(&bars->kv_empty[slot]);      // (tile 1 walks no fewer blocks than tile 0)
+        if (kOneS || t == 1) ptx::tcgen05_commit(&bars->kv_empty[slot]);     // (tile 1 walks no fewer blocks than tile 0)
       }
       __syncwarp();
       return true;
@@ -256,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_attn_kernel(const __grid_co
     // per MMA), V MN-major (D contiguous): 16 key rows per MMA = 2048 bytes down a block, blocks of 64 head-dim columns 16 KiB
     // apart
     auto values = [&](int t, int j) {
-      const int v_item = 2 * item_of(t, j) + 1, slot = v_item % kSlots;
+      const int v_item = 2 * j + 1, slot = v_item % kSlots;
       const uint32_t vl = v_lo + static_cast<uint32_t>(slot * (kSlotBytes >> 4));
       if (first_use(t, j) && !wait_item(v_item)) return false;
       constexpr int kParts = kOneS ? 1 : 2, kPerPart = kBKV / 16 / kParts;
@@ -271,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1) flash_attn_kernel(const __grid_co
                              p.idesc_pv, (j > 0 || kk != 0) ? 1u : 0u);
           if (part + 1 == kParts) {
             ptx::tcgen05_commit(j + 1 < nblk[t] ? &bars->pv_done[t] : &bars->o_done[t]);
-            if (last_use(t, j)) ptx::tcgen05_commit(&bars->kv_empty[slot]);
+            if (kOneS || t == 1) ptx::tcgen05_commit(&bars->kv_empty[slot]);
           }
         }
         __syncwarp();
@@ -287,14 +259,13 @@ __global__ void __launch_bounds__(kThreads, 1) flash_attn_kernel(const __grid_co
         ok = ok && values(t, j);
       }
       // the other tile walks on: its blocks are released for this one too, each when it has arrived
-      // (with `skip` no later block waits for the two that one tile leaves out)
-      for (int item = 2 * nt; ok && !(WINDOW && skip) && item < 2 * nmax; ++item) {
+      for (int item = 2 * nt; ok && item < 2 * nmax; ++item) {
         ok = wait_item(item);
         if (ok && lane == 0) ptx::mbar_arrive(&bars->kv_empty[item % kSlots]);
       }
     } else {
       ok = ok && scores(0, 0) && scores(1, 0);
-      for (int j = 0; ok && j < nblk[1]; ++j) {
+      for (int j = 0; ok && j < nmax; ++j) {
 #pragma unroll
         for (int t = 0; t < kTiles; ++t)
           if (j + 1 < nblk[t]) ok = ok && scores(t, j + 1);
@@ -317,27 +288,20 @@ __global__ void __launch_bounds__(kThreads, 1) flash_attn_kernel(const __grid_co
     const int n_mine = nblk[t];
     const int vis = p.causal ? min(p.Sk, qi % p.pos + shift + 1) : p.Sk;    // keys [0, vis) are visible to this row
     const int vis_tile = p.causal ? min(p.Sk, tile_lo(t) + shift + 1) : p.Sk;   // ... to every row of the tile
-    [[maybe_unused]] const int win_tile = WINDOW ? min(p.Sk - 1, tile_hi(t) + shift) - p.window : 0;   // a key past it is in every row's window, up to the row
     const float sc = p.scale_log2;
     RowState st;
     bool ok = true;
     for (int j = 0; j < n_mine; ++j) {
       if (!ptx::mbar_wait(&bars->s_full[t], static_cast<uint32_t>(j & 1), p.timeout_ns, abort_flag)) { ok = false; break; }
       ptx::tcgen05_fence_after();
-      const int key0 = block_of(j0 + item_of(t, j)) * kBKV;
+      const int key0 = (j0 + j) * kBKV;
       // masked: some row of the tile does not see all of the block
       // P V of block j - 1 has read P, and O is whole
       auto previous = [&] {
         if (j > 0 && !ptx::mbar_wait(&bars->pv_done[t], static_cast<uint32_t>(j - 1) & 1u, p.timeout_ns, abort_flag)) ok = false;
         ptx::tcgen05_fence_after();
       };
-      bool masked = key0 + kBKV > vis_tile;
-      if constexpr (WINDOW) masked = masked || (key0 <= win_tile && key0 + kBKV > p.sinks);
-      auto mask = [&] {
-        if constexpr (WINDOW) return WindowMask{vis - key0, qi % p.pos + shift - p.window + 1 - key0, p.sinks - key0};
-        else return vis - key0;
-      }();
-      softmax_row_block<FMT>(t_s, t_p, masked, mask, sc, st, [&] {
+      softmax_row_block<FMT>(t_s, t_p, key0 + kBKV > vis_tile, vis - key0, sc, st, [&] {
         ptx::tcgen05_fence_before();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&bars->s_free[t]);
@@ -458,19 +422,13 @@ struct AttnPlan {
   double load;         // key blocks of the busiest SM
 };
 
-AttnPlan attn_plan(int B, int Hq, int Hk, int Sq, int Sk, int causal, bool cut, int window = 0, int sinks = 0) {
+AttnPlan attn_plan(int B, int Hq, int Hk, int Sq, int Sk, int causal, bool cut) {
   const int group = Hq / Hk, rows_cta = attn::kTiles * attn::kBQ, pos = Sq;
-  auto blocks = [&](int hi, int span) {
-    const int64_t end = causal ? std::min<int64_t>(Sk, static_cast<int64_t>(hi) + Sk - pos) : Sk;
-    // (windowed: the blocks that the windows of `span` positions reach and those of the sinks, all before `end` at most)
-    const int64_t most = window > 0 ? static_cast<int64_t>(window) + span + 127 + (static_cast<int64_t>(sinks) + 127) / 128 * 128 : end;
-    return static_cast<double>(std::min(end, most) + 127) / 128;
-  };
-  // (packed, the rows of a CTA may be the end of one head and the start of the next: all positions)
-  const double longest = blocks(pos, std::min(rows_cta, pos)), longest_packed = blocks(pos, pos);
+  auto blocks = [&](int hi) { return static_cast<double>((causal ? std::min<int64_t>(Sk, static_cast<int64_t>(hi) + Sk - pos) : Sk) + 127) / 128; };
+  const double longest = blocks(pos);
   AttnPlan d{Hq, Sq, (Sq + rows_cta - 1) / rows_cta, 1, 0, 0.0}, packed = d;
   double plain = 0.0;
-  for (int i = 0; i < d.tiles; ++i) plain += blocks(std::min((i + 1) * rows_cta, pos), std::min(rows_cta, pos));
+  for (int i = 0; i < d.tiles; ++i) plain += blocks(std::min((i + 1) * rows_cta, pos));
   d.load = std::max(longest, static_cast<double>(B) * Hq * plain / 148.0);
   bool pack = false;
   // A call of few query positions: the query heads of a KV head are contiguous rows, so they can fill tiles together. It
@@ -482,19 +440,19 @@ AttnPlan attn_plan(int B, int Hq, int Hk, int Sq, int Sk, int causal, bool cut, 
     packed.Hq = Hk;
     packed.tiles = (packed.Sq + rows_cta - 1) / rows_cta;
     pack = true;
-    packed.load = std::max(longest_packed, static_cast<double>(B) * Hk * packed.tiles * longest_packed / 148.0);
+    packed.load = std::max(longest, static_cast<double>(B) * Hk * packed.tiles * longest / 148.0);
     if (packed.load < 0.95 * d.load) d = packed;
   }
   // Few tiles over many keys leave SMs idle: the keys are then cut into slices, which a second kernel merges. In us, a CTA takes 5
   // and 1.55 a block of keys, the merge 4 and its bytes at 3 TB/s. In a loop, D = 128: 32 heads x 131 positions over 3404 keys 46 ->
   // 26 us, 256 over 4096 54 -> 26, 8 heads x 512 over 16384 199 -> 40, 4 x 4096 causal 54 -> 39. Below 14 blocks a call waits
   // for its host work, which the second launch makes longer (8 blocks 17.0 -> 20.0 us, 12 blocks 22.9 -> 24.0).
+  const int nblk = (Sk + 127) / 128;
   if (!cut || longest < 14.0) return d;
   double best = 0.85 * (5.0 + 1.55 * longest);
   const AttnPlan forms[2] = {d, packed};
   for (int f = 0; f < (pack ? 2 : 1); ++f) {
     const AttnPlan& x = forms[f];
-    const int nblk = window > 0 ? static_cast<int>(x.Hq == Hq ? longest : longest_packed) : (Sk + 127) / 128;
     const int64_t ctas = static_cast<int64_t>(B) * x.Hq * x.tiles, rows = static_cast<int64_t>(B) * x.Hq * x.Sq;
     for (int n = 2; n <= 16 && ctas * n <= 148 && 2 * n <= nblk; ++n) {
       const int per = (nblk + n - 1) / n, slices = (nblk + per - 1) / per;
@@ -507,19 +465,10 @@ AttnPlan attn_plan(int B, int Hq, int Hk, int Sq, int Sk, int causal, bool cut, 
 }  // namespace
 
 // Scratch of a call whose keys are cut into slices, else 0
-static int64_t attention_scratch(int B, int Hq, int Hk, int Sq, int Sk, int D, int causal, int window, int sinks) {
-  if (B <= 0 || Hq <= 0 || Hk <= 0 || Sq <= 0 || Sk <= 0 || Hq % Hk != 0 || (D != 64 && D != 128)) return 0;
-  const AttnPlan d = attn_plan(B, Hq, Hk, Sq, Sk, causal, true, window, sinks);
-  return d.slices > 1 ? static_cast<int64_t>(d.slices) * B * Hq * Sq * (D + 2) * static_cast<int64_t>(sizeof(float)) : 0;
-}
-
 extern "C" int64_t catcoc_flash_attention_workspace_bytes(int B, int Hq, int Hk, int Sq, int Sk, int D, int causal) {
-  return attention_scratch(B, Hq, Hk, Sq, Sk, D, causal, 0, 0);
-}
-
-extern "C" int64_t catcoc_window_route(int B, int Hq, int Hk, int Sq, int Sk, int D, int window, int sinks) {
-  const int64_t decode = catcoc_window_decode_workspace_bytes(B, Hq, Hk, Sq, Sk, D, window, sinks);
-  return decode >= 0 ? decode : -1 - attention_scratch(B, Hq, Hk, Sq, Sk, D, 1, window, sinks);
+  if (B <= 0 || Hq <= 0 || Hk <= 0 || Sq <= 0 || Sk <= 0 || Hq % Hk != 0 || (D != 64 && D != 128)) return 0;
+  const AttnPlan d = attn_plan(B, Hq, Hk, Sq, Sk, causal, true);
+  return d.slices > 1 ? static_cast<int64_t>(d.slices) * B * Hq * Sq * (D + 2) * static_cast<int64_t>(sizeof(float)) : 0;
 }
 
 extern "C" int64_t catcoc_attention_route(int B, int Hq, int Hk, int Sq, int Sk, int D, int causal) {
@@ -533,8 +482,9 @@ extern "C" int catcoc_flash_attention(const void* q, const void* k, const void* 
   return catcoc_flash_attention_cut(q, k, v, out, nullptr, B, Hq, Hk, Sq, Sk, D, fmt, causal, scale, status, timeout_ns, stream);
 }
 
-static int attention_call(const void* q, const void* k, const void* v, void* out, void* workspace, int B, int Hq, int Hk, int Sq, int Sk, int D, int fmt,
-                          int causal, float scale, uint32_t* status, uint64_t timeout_ns, void* stream, int window, int sinks) {
+extern "C" int catcoc_flash_attention_cut(const void* q, const void* k, const void* v, void* out, void* workspace, int B, int Hq, int Hk,
+                                          int Sq, int Sk, int D, int fmt, int causal, float scale, uint32_t* status,
+                                          uint64_t timeout_ns, void* stream) {
   if (!q || !k || !v || !out || !status || B <= 0 || Hq <= 0 || Hk <= 0 || Sq <= 0 || Sk <= 0) {
     set_error("flash_attention: bad arguments");
     return CATCOC_E_BAD_ARG;
@@ -545,7 +495,7 @@ static int attention_call(const void* q, const void* k, const void* v, void* out
   if (causal && Sk < Sq) { set_error("causal attention needs Sk >= Sq"); return CATCOC_E_BAD_ARG; }
   if (!(scale > 0.0f)) { set_error("flash_attention: the softmax scale must be positive (the row maximum is taken before scaling)"); return CATCOC_E_UNSUPPORTED; }
   const int rows_cta = attn::kTiles * attn::kBQ, pos = Sq;
-  const AttnPlan d = attn_plan(B, Hq, Hk, Sq, Sk, causal, workspace != nullptr, window, sinks);
+  const AttnPlan d = attn_plan(B, Hq, Hk, Sq, Sk, causal, workspace != nullptr);
   Hq = d.Hq;
   Sq = d.Sq;
   attn::AttnParams p;
@@ -560,7 +510,6 @@ static int attention_call(const void* q, const void* k, const void* v, void* out
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = workspace != nullptr ? p.part_o + d.slices * rows * D : nullptr;
   p.per = d.per;
-  p.window = window; p.sinks = sinks;
   p.B = B; p.Hq = Hq; p.Hk = Hk; p.Sq = Sq; p.Sk = Sk; p.D = D; p.pos = pos;
   const int64_t ctas = static_cast<int64_t>(B) * Hq * ((Sq + rows_cta - 1) / rows_cta);
   if (ctas > 0x7fffffff) { set_error("flash_attention: too many query tiles"); return CATCOC_E_TOO_LARGE; }
@@ -598,40 +547,19 @@ static int attention_call(const void* q, const void* k, const void* v, void* out
   const bool bf = fmt == CATCOC_FMT_BF16;
   int lrc;
   if (d.slices > 1) {
-    if (window > 0 && D == 128) lrc = bf ? launch(attn::flash_attn_kernel<128, FMT_BF16, true, true, true>) : launch(attn::flash_attn_kernel<128, FMT_F16, true, true, true>);
-    else if (window > 0) lrc = bf ? launch(attn::flash_attn_kernel<64, FMT_BF16, true, true, true>) : launch(attn::flash_attn_kernel<64, FMT_F16, true, true, true>);
-    else if (D == 128) lrc = bf ? launch(attn::flash_attn_kernel<128, FMT_BF16, true, true, false>) : launch(attn::flash_attn_kernel<128, FMT_F16, true, true, false>);
-    else lrc = bf ? launch(attn::flash_attn_kernel<64, FMT_BF16, true, true, false>) : launch(attn::flash_attn_kernel<64, FMT_F16, true, true, false>);
+    if (D == 128) lrc = bf ? launch(attn::flash_attn_kernel<128, FMT_BF16, true, true>) : launch(attn::flash_attn_kernel<128, FMT_F16, true, true>);
+    else lrc = bf ? launch(attn::flash_attn_kernel<64, FMT_BF16, true, true>) : launch(attn::flash_attn_kernel<64, FMT_F16, true, true>);
     if (lrc == 0 && D == 128) lrc = bf ? merge(attn::flash_slices_kernel<128, FMT_BF16>) : merge(attn::flash_slices_kernel<128, FMT_F16>);
     else if (lrc == 0) lrc = bf ? merge(attn::flash_slices_kernel<64, FMT_BF16>) : merge(attn::flash_slices_kernel<64, FMT_F16>);
-  } else if (window > 0) {
-    if (D == 128) lrc = bf ? launch(attn::flash_attn_kernel<128, FMT_BF16, false, true, true>) : launch(attn::flash_attn_kernel<128, FMT_F16, false, true, true>);
-    else lrc = bf ? launch(attn::flash_attn_kernel<64, FMT_BF16, false, true, true>) : launch(attn::flash_attn_kernel<64, FMT_F16, false, true, true>);
   } else if (D == 128) {
-    lrc = bf ? launch(attn::flash_attn_kernel<128, FMT_BF16, false, true, false>) : launch(attn::flash_attn_kernel<128, FMT_F16, false, true, false>);
+    lrc = bf ? launch(attn::flash_attn_kernel<128, FMT_BF16, false, true>) : launch(attn::flash_attn_kernel<128, FMT_F16, false, true>);
   } else if (late_wait(d.load, ctas, causal, pos, Sk)) {
-    lrc = bf ? launch(attn::flash_attn_kernel<64, FMT_BF16, false, true, false>) : launch(attn::flash_attn_kernel<64, FMT_F16, false, true, false>);
+    lrc = bf ? launch(attn::flash_attn_kernel<64, FMT_BF16, false, true>) : launch(attn::flash_attn_kernel<64, FMT_F16, false, true>);
   } else {
-    lrc = bf ? launch(attn::flash_attn_kernel<64, FMT_BF16, false, false, false>) : launch(attn::flash_attn_kernel<64, FMT_F16, false, false, false>);
+    lrc = bf ? launch(attn::flash_attn_kernel<64, FMT_BF16, false, false>) : launch(attn::flash_attn_kernel<64, FMT_F16, false, false>);
   }
   if (lrc != 0) return lrc;
   e = cudaGetLastError();
   if (e != cudaSuccess) { set_error("flash_attention launch failed: %s", cudaGetErrorString(e)); return -1000 - static_cast<int>(e); }
   return CATCOC_OK;
-}
-
-extern "C" int catcoc_flash_attention_cut(const void* q, const void* k, const void* v, void* out, void* workspace, int B, int Hq, int Hk,
-                                          int Sq, int Sk, int D, int fmt, int causal, float scale, uint32_t* status,
-                                          uint64_t timeout_ns, void* stream) {
-  return attention_call(q, k, v, out, workspace, B, Hq, Hk, Sq, Sk, D, fmt, causal, scale, status, timeout_ns, stream, 0, 0);
-}
-
-extern "C" int catcoc_window_attention(const void* q, const void* k, const void* v, void* out, void* workspace, int B, int Hq, int Hk, int Sq, int Sk, int D,
-                                       int fmt, int window, int sinks, float scale, uint32_t* status, uint64_t timeout_ns, void* stream) {
-  if (window < 1 || sinks < 0) { set_error("window_attention: a window of at least 1 and no negative sinks"); return CATCOC_E_BAD_ARG; }
-  window = std::min(window, 1 << 30);                              // (both beyond any length; their sums stay in range)
-  sinks = std::min(sinks, 1 << 30);
-  if (catcoc_window_decode_workspace_bytes(B, Hq, Hk, Sq, Sk, D, window, sinks) >= 0)
-    return catcoc_window_decode(q, k, v, out, workspace, B, Hq, Hk, Sq, Sk, D, fmt, window, sinks, scale, status, timeout_ns, stream);
-  return attention_call(q, k, v, out, workspace, B, Hq, Hk, Sq, Sk, D, fmt, 1, scale, status, timeout_ns, stream, window, sinks);
 }
