@@ -9,6 +9,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <type_traits>
 #include "catcoc/params.h"
 #include "catcoc/ptx.cuh"
 
@@ -25,12 +26,28 @@ CATCOC_DEVICE uint32_t pack16(float lo, float hi) {
 }
 
 // Which scores of a block a row does not see: those from key `vis_left` on, or, with a window, also those in front of its first key
-// that are none of the first `sinks` (all counted from the block's first key).
+// that are none of the first `sinks` (all counted from the block's first key). A window's are kept as bits, which are tested by one
+// instruction where the three bounds would take three.
+CATCOC_DEVICE uint32_t low_bits(int n) {                     // the lowest n, none below 0, all from 32 on
+  uint32_t r;
+  asm("bmsk.clamp.b32 %0, 0, %1;" : "=r"(r) : "r"(max(n, 0)));
+  return r;
+}
 struct WindowMask {
-  int vis_left, first, sinks;
+  uint32_t seen[kRowKeys / 32];
+  CATCOC_DEVICE WindowMask(int vis_left, int first, int sinks) {
+#pragma unroll
+    for (int c = 0; c < kRowKeys / 32; ++c)
+      seen[c] = low_bits(vis_left - 32 * c) & (~low_bits(first - 32 * c) | low_bits(sinks - 32 * c));
+  }
 };
+// A mask, or a function that makes it where it is needed
+template <class T> CATCOC_DEVICE auto mask_of(T&& t) {
+  if constexpr (std::is_invocable_v<T>) return t();
+  else return t;
+}
 CATCOC_DEVICE bool hides(int vis_left, int i) { return i >= vis_left; }
-CATCOC_DEVICE bool hides(const WindowMask& w, int i) { return i >= w.vis_left || (i < w.first && i >= w.sinks); }
+CATCOC_DEVICE bool hides(const WindowMask& w, int i) { return (w.seen[i >> 5] & (1u << (i & 31))) == 0u; }
 
 // m: reference maximum (log2 domain), l: running sum
 struct RowState {
@@ -55,12 +72,12 @@ CATCOC_DEVICE void rescale_o(uint32_t t_o, float alpha) {
 // place, and updates the state. `loaded()` is called when the scores are in registers, `before(move, alpha)` ahead of the
 // first probability: with `move` (the same in all lanes) the reference maximum of some row of the warp moved and O has to
 // be multiplied by alpha; `ready()` ahead of the first store of probabilities, `half()` behind
-// it (those of the first 64 keys). `mask`: the keys of this block the row sees (used when `masked`), a number of them or a WindowMask.
+// it (those of the first 64 keys). `make_mask`: the keys of this block the row sees (used when `masked`): a number of them, or a function that gives a WindowMask.
 //
 // Tried and not kept: a quarter of the exponentials as a degree-5 polynomial on the FMA pipe (D = 128, causal 4 % faster, not causal 2
 // to 6 % slower, D = 64 slower), the two warps of a scheduler taking their exponentials strictly in turn (4 % slower).
-template <int FMT, class Mask, class Loaded, class Before, class Ready, class Half>
-CATCOC_DEVICE void softmax_row_block(uint32_t t_s, uint32_t t_p, bool masked, Mask mask, float sc, RowState& st, Loaded&& loaded,
+template <int FMT, class MakeMask, class Loaded, class Before, class Ready, class Half>
+CATCOC_DEVICE void softmax_row_block(uint32_t t_s, uint32_t t_p, bool masked, MakeMask&& make_mask, float sc, RowState& st, Loaded&& loaded,
                                      Before&& before, Ready&& ready, Half&& half) {
   uint32_t v[4][32];
 #pragma unroll
@@ -68,6 +85,7 @@ CATCOC_DEVICE void softmax_row_block(uint32_t t_s, uint32_t t_p, bool masked, Ma
   ptx::tcgen05_wait_ld();
   loaded();
   if (masked) {
+    const auto mask = mask_of(make_mask);
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll

@@ -248,9 +248,9 @@ __global__ void __launch_bounds__(kThreads, 1) flash_decode_kernel(const __grid_
         bool masked = key0 + kBKV > vis_all;
         if constexpr (WINDOW) masked = masked || (key0 <= p.Sk - 1 - p.window && key0 + kBKV > p.sinks);
         auto mask = [&] {
-          if constexpr (WINDOW) return attn::WindowMask{vis - key0, vis - p.window - key0, p.sinks - key0};   // (vis - 1 is the row's position)
+          if constexpr (WINDOW) return attn::WindowMask(vis - key0, vis - p.window - key0, p.sinks - key0);   // (vis - 1 is the row's position)
           else return vis - key0;
-        }();
+        };
         attn::softmax_row_block<FMT>(t_s, t_s, masked, mask, p.scale_log2, st, [] {}, [&](bool move, float alpha) {
           // s_full(i) was committed behind the second product of this parity's previous block, so O_t is whole
           if (move && i > mine0) attn::rescale_o<D>(t_o, alpha);

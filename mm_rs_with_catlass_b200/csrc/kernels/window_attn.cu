@@ -42,6 +42,19 @@ constexpr int kProducerWarp = 8, kIssuerWarp = 9;
 constexpr int kBlockBytes = 128 * 128;               // one 128-row x 128-byte (64 element) swizzled block
 constexpr int kMaxSlots = 8;
 
+// Division of numbers below 2^31 by a number that the host knows: n / d = n m >> (31 + s) with d <= 2^s and m = 2^(31 + s) / d + 1. The
+// divisions of a piece of work were a chain of thousands of cycles in front of its first block (window 128: 11.1 us a piece).
+struct Divisor {
+  uint32_t d, m, s;
+  void set(uint32_t by) {
+    d = by;
+    for (s = 0; (1u << s) < by; ++s) {}
+    m = static_cast<uint32_t>((1ull << (31 + s)) / by + 1ull);
+  }
+  CATCOC_DEVICE int div(int n) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * m) >> (31u + s)); }
+  CATCOC_DEVICE int mod(int n) const { return n - div(n) * static_cast<int>(d); }
+};
+
 struct WindowParams {
   CUtensorMap tm_q, tm_k, tm_v;   // {D, S, B * H} with a {64, 128, 1} box, 128-byte swizzle
   void* out;                      // [B, Hq, Sq, D]
@@ -49,6 +62,7 @@ struct WindowParams {
   int pos;                        // query positions: row r stands at r % pos
   int window, sinks;
   int tiles, works, slices;       // pieces of work a head, in all, and slices of each
+  Divisor by_works, by_heads, by_hq, by_group, by_pos;   // works, B * Hq, Hq, Hq / Hk, pos
   float scale_log2;               // softmax scale * log2(e), > 0
   uint32_t idesc_qk, idesc_pv;
   uint32_t* status;
@@ -81,19 +95,19 @@ struct Work {
   int lo[kTiles], hi[kTiles];              // positions of a tile's rows
 
   CATCOC_DEVICE Work(const WindowParams& p, int index) {
-    slice = CUT ? index / p.works : 0;
+    slice = CUT ? p.by_works.div(index) : 0;
     const int w = index - slice * p.works, heads = p.B * p.Hq;
     // heads side by side, so that those of a KV head meet its blocks in the L2; the early tiles, which see less, last
-    const int qt = p.tiles - 1 - w / heads;
-    bh = w % heads;
+    const int early = p.by_heads.div(w), qt = p.tiles - 1 - early;
+    bh = w - early * heads;
     q0 = qt * (kTiles * kBQ);
-    const int b = bh / p.Hq;
-    bhk = b * p.Hk + (bh - b * p.Hq) / (p.Hq / p.Hk);
+    const int b = p.by_hq.div(bh);
+    bhk = b * p.Hk + p.by_group.div(bh - b * p.Hq);
     const int shift = p.Sk - p.pos;
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
       // (all positions when the rows of two packed heads meet in the tile; a tile without rows does as the other)
-      const int r = (q0 + (t == 1 && q0 + kBQ >= p.Sq ? 0 : t * kBQ)) % p.pos;
+      const int r = p.by_pos.mod(q0 + (t == 1 && q0 + kBQ >= p.Sq ? 0 : t * kBQ));
       const bool wrap = r + kBQ > p.pos && p.pos < p.Sq;
       lo[t] = (wrap ? 0 : r) + shift;
       hi[t] = min(wrap ? p.pos - 1 : r + kBQ - 1, p.pos - 1) + shift;
@@ -119,6 +133,13 @@ struct Work {
     if (item < sink_blocks) return item;
     if (!skip) return first + item - sink_blocks;
     return item == shared ? first : first + item - sink_blocks + (item < shared ? 1 : 0);
+  }
+  // The tile's blocks that all of its rows see whole: the first `sinks_end` and [begin, end) of those it walks, at least
+  CATCOC_DEVICE void whole(const WindowParams& p, int t, int& sinks_end, int& begin, int& end) const {
+    const int ahead = sink_blocks - first - (skip ? 1 : 0) - j0;         // walked as the (block + ahead)-th
+    sinks_end = min(p.sinks / kBKV, sink_blocks) - j0;
+    begin = max(sink_blocks - j0, (hi[t] >= p.window ? (hi[t] - p.window) / kBKV + 1 : 0) + ahead);
+    end = (lo[t] + 1) / kBKV + ahead;
   }
   CATCOC_DEVICE int item_of(int t, int j) const { return skip && t == 1 && j == shared ? j + 1 : j; }
 };
@@ -334,22 +355,33 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
     bool ok = true;
     uint32_t c = 0;                                  // blocks of this tile since the start
     for (int index = blockIdx.x; ok && index < total; index += gridDim.x) {
-      const Work<CUT> w(p, index);
-      const int qi = w.q0 + t * kBQ + qd * 32 + lane;      // query row inside the head
-      const int n_mine = w.nblk[t], mine = qi % p.pos + p.Sk - p.pos;   // position of this row
+      // (only what every block needs stays in registers, which hold the row's 128 scores; the rest is worked out where it is needed)
+      int n_mine, sinks_end, begin, end;
+      {
+        const Work<CUT> w(p, index);
+        n_mine = w.nblk[t];
+        w.whole(p, t, sinks_end, begin, end);
+      }
+      auto again = [&] {
+        int same = index;
+        asm volatile("" : "+r"(same));
+        return Work<CUT>(p, same);
+      };
       RowState st;
       for (int j = 0; j < n_mine; ++j, ++c) {
         if (!ptx::mbar_wait(&bars->s_full[t], c & 1u, p.timeout_ns, abort_flag)) { ok = false; break; }
         ptx::tcgen05_fence_after();
-        const int key0 = w.block_of(w.item_of(t, j)) * kBKV;
         // P V of the block before has read P, and O is whole
         auto previous = [&] {
           if (j > 0 && !ptx::mbar_wait(&bars->pv_done[t], (c - 1u) & 1u, p.timeout_ns, abort_flag)) ok = false;
           ptx::tcgen05_fence_after();
         };
-        // masked: some row of the tile does not see all of the block
-        const bool masked = key0 + kBKV - 1 > w.lo[t] || (key0 <= w.hi[t] - p.window && key0 + kBKV > p.sinks);
-        const attn::WindowMask mask{mine + 1 - key0, mine - p.window + 1 - key0, p.sinks - key0};
+        const bool masked = j >= sinks_end && (j < begin || j >= end);
+        auto mask = [&] {
+          const Work<CUT> w = again();
+          const int key0 = w.block_of(w.item_of(t, j)) * kBKV, mine = p.by_pos.mod(w.q0 + t * kBQ + qd * 32 + lane) + p.Sk - p.pos;
+          return attn::WindowMask(mine + 1 - key0, mine - p.window + 1 - key0, p.sinks - key0);
+        };
         attn::softmax_row_block<FMT>(t_s, t_p, masked, mask, sc, st, [&] {
           ptx::tcgen05_fence_before();
           __syncwarp();
@@ -377,6 +409,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       if (!ok) break;
       ptx::tcgen05_fence_after();
       const float inv = (st.l > 0.0f) ? 1.0f / st.l : 0.0f;
+      const Work<CUT> w = again();
+      const int qi = w.q0 + t * kBQ + qd * 32 + lane;      // query row inside the head
       uint8_t* orow = static_cast<uint8_t*>(p.out) + (static_cast<int64_t>(w.bh) * p.Sq + qi) * D * 2;
 #pragma unroll
       for (int col = 0; col < D / 32; ++col) {
@@ -544,6 +578,11 @@ extern "C" int catcoc_window_attention(const void* q, const void* k, const void*
   p.B = B; p.Hq = Hq; p.Hk = Hk; p.Sq = Sq; p.Sk = Sk; p.pos = pos;
   p.window = window; p.sinks = sinks;
   p.tiles = d.tiles; p.works = static_cast<int>(works); p.slices = d.slices; p.per = d.per;
+  p.by_works.set(static_cast<uint32_t>(works));
+  p.by_heads.set(static_cast<uint32_t>(B) * Hq);
+  p.by_hq.set(static_cast<uint32_t>(Hq));
+  p.by_group.set(static_cast<uint32_t>(Hq / Hk));
+  p.by_pos.set(static_cast<uint32_t>(pos));
   p.scale_log2 = scale * 1.4426950408889634f;
   const uint32_t f = fmt == CATCOC_FMT_BF16 ? 1u : 0u;
   p.idesc_qk = ptx::make_instr_desc(1u, f, f, 0u, 0u, 128u, 128u);
