@@ -143,6 +143,11 @@ CATCOC_DEVICE void tma_store_2d(const void* tmap, uint32_t smem_src, int x, int 
                ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(smem_src), "r"(x), "r"(y)
                : "memory");
 }
+CATCOC_DEVICE void tma_store_3d(const void* tmap, uint32_t smem_src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];"
+               ::"l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(smem_src)
+               : "memory");
+}
 CATCOC_DEVICE void bulk_commit_group() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // Waits until at most N of this thread's bulk groups still READ their shared-memory source.
 template <int N>

@@ -3,7 +3,8 @@
 // A tile of 128 query rows sees window + 128 keys at most, a few blocks of 128, where a causal tile sees up to all of them. So
 // what a CTA does besides its blocks counts: with a launch's CTAs one after the other, 1 x 32 / 8 heads x 8192 took 1.67 us a block and
 // 8.3 us a CTA (TMEM, barriers, the first copies and products, the last ones, the store). Here an SM keeps one CTA, which
-// takes every 148th piece of work: the copies run on into the next one, and its first scores are computed under the softmax of the last block.
+// takes every 148th piece of work: the copies run on into the next one, its first scores are computed under the last block's end, and the
+// output leaves by TMA while it is worked on. (First scores ahead of the last block's product with V waited for the next queries: 117 -> 124 us.)
 //
 //   warps 0..3, 4..7  softmax of tile 0, tile 1: one query row per thread (softmax_row.cuh)
 //   warp 8            TMA producer: Q tiles, K and V blocks of 128 keys through one ring of slots
@@ -41,6 +42,7 @@ constexpr int kSoftmaxRegs = 216, kOtherRegs = 72;   // of 168 a thread: 2 x 216
 constexpr int kProducerWarp = 8, kIssuerWarp = 9;
 constexpr int kBlockBytes = 128 * 128;               // one 128-row x 128-byte (64 element) swizzled block
 constexpr int kMaxSlots = 8;
+constexpr int kOutBytes = 8 * 32 * 128;
 
 // Division of numbers below 2^31 by a number that the host knows: n / d = n m >> (31 + s) with d <= 2^s and m = 2^(31 + s) / d + 1. The
 // divisions of a piece of work were a chain of thousands of cycles in front of its first block (window 128: 11.1 us a piece).
@@ -57,7 +59,7 @@ struct Divisor {
 
 struct WindowParams {
   CUtensorMap tm_q, tm_k, tm_v;   // {D, S, B * H} with a {64, 128, 1} box, 128-byte swizzle
-  void* out;                      // [B, Hq, Sq, D]
+  CUtensorMap tm_o;               // out {D, Sq, B * Hq} with a {64, 32, 1} box: a warp's rows, of which those past Sq are not written
   int B, Hq, Hk, Sq, Sk;          // Sq: rows per (batch, query head), or per (batch, KV head) when its heads are packed
   int pos;                        // query positions: row r stands at r % pos
   int window, sinks;
@@ -159,7 +161,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint8_t* sq = smem;                            // two Q tiles
   uint8_t* skv = sq + kTiles * kQBytes;
-  Bars* bars = reinterpret_cast<Bars*>(skv + kSlots * kSlotBytes);
+  uint8_t* sout = skv + kSlots * kSlotBytes;     // of each softmax warp, 32 rows x 64 columns on their way out
+  Bars* bars = reinterpret_cast<Bars*>(sout + kOutBytes);
   volatile uint32_t* abort_flag = &bars->abort_flag;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int total = p.works * p.slices;
@@ -292,56 +295,34 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       }
       return true;
     };
-    auto behind = [](const Work<CUT>& w, Before f) {
-      ++f.count;
-      f.base += 2u * static_cast<uint32_t>(w.items);
-      f.c[0] += static_cast<uint32_t>(w.nblk[0]);
-      f.c[1] += static_cast<uint32_t>(w.nblk[1]);
-      return f;
-    };
-    bool ok = true, begun = false;                 // `begun`: the first scores of the piece were issued ahead
+    bool ok = true;
     Before f{0u, 0u, {0u, 0u}};
     for (int index = blockIdx.x; ok && index < total; index += gridDim.x) {
       const Work<CUT> w(p, index);
-      const int next = index + static_cast<int>(gridDim.x);
       if constexpr (kOneS) {
         const int t = warp - kIssuerWarp, nt = w.nblk[t];
-        // Items behind the tile's last one, which it passes on: at most one here, or the tile would wait for blocks that wait for it
-        const int rest = t == 1 ? 0 : w.items - nt;
-        if (!begun) ok = scores(w, f, t, 0);
-        begun = false;
+        ok = scores(w, f, t, 0);
         for (int j = 0; ok && j < nt; ++j) {
-          // ahead of the product with V, which waits for this block's softmax: the next block's scores, or the next piece's first
-          if (j + 1 < nt) {
-            ok = scores(w, f, t, j + 1);
-          } else if (next < total && rest <= 1) {
-            if (rest == 1) ok = pass(f.base + 2u * static_cast<uint32_t>(nt));
-            ok = ok && scores(Work<CUT>(p, next), behind(w, f), t, 0);
-            begun = true;
-          }
+          if (j + 1 < nt) ok = scores(w, f, t, j + 1);      // ahead of the product with V, which waits for this block's softmax
           ok = ok && values(w, f, t, j);
         }
-        for (int i = begun && rest == 1 ? 2 * nt + 1 : 2 * nt; ok && t == 0 && i < 2 * w.items; ++i) ok = pass(f.base + static_cast<uint32_t>(i));
+        // items behind tile 0's last one
+        for (int i = 2 * nt; ok && t == 0 && i < 2 * w.items; ++i) ok = pass(f.base + static_cast<uint32_t>(i));
       } else {
-        if (!begun) ok = scores(w, f, 0, 0) && scores(w, f, 1, 0);
-        begun = false;
+        ok = scores(w, f, 0, 0) && scores(w, f, 1, 0);
         for (int j = 0; ok && j < w.nblk[1]; ++j) {
-          if (j + 1 < w.nblk[1]) {
 #pragma unroll
-            for (int t = 0; t < kTiles; ++t)
-              if (j + 1 < w.nblk[t]) ok = ok && scores(w, f, t, j + 1);
-          } else if (next < total) {
-            const Work<CUT> ahead(p, next);
-            const Before g = behind(w, f);
-            ok = scores(ahead, g, 0, 0) && scores(ahead, g, 1, 0);
-            begun = true;
-          }
+          for (int t = 0; t < kTiles; ++t)
+            if (j + 1 < w.nblk[t]) ok = ok && scores(w, f, t, j + 1);
 #pragma unroll
           for (int t = 0; t < kTiles; ++t)
             if (j < w.nblk[t]) ok = ok && values(w, f, t, j);
         }
       }
-      f = behind(w, f);
+      ++f.count;
+      f.base += 2u * static_cast<uint32_t>(w.items);
+      f.c[0] += static_cast<uint32_t>(w.nblk[0]);
+      f.c[1] += static_cast<uint32_t>(w.nblk[1]);
     }
     if (!ok && lane == 0) { fail(p, 2u, 0u); *abort_flag = 1; }
   } else if (warp < kProducerWarp) {
@@ -410,26 +391,42 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       ptx::tcgen05_fence_after();
       const float inv = (st.l > 0.0f) ? 1.0f / st.l : 0.0f;
       const Work<CUT> w = again();
-      const int qi = w.q0 + t * kBQ + qd * 32 + lane;      // query row inside the head
-      uint8_t* orow = static_cast<uint8_t*>(p.out) + (static_cast<int64_t>(w.bh) * p.Sq + qi) * D * 2;
+      const int row0 = w.q0 + t * kBQ + qd * 32;           // this warp's first query row inside the head
 #pragma unroll
       for (int col = 0; col < D / 32; ++col) {
         uint32_t v[32];
         ptx::tmem_ld_32x32b_x32(t_o + col * 32, v);
         ptx::tcgen05_wait_ld();
-        if (CUT && qi < p.Sq) {
-          const int64_t prow = (static_cast<int64_t>(w.slice) * p.B * p.Hq + w.bh) * p.Sq + qi;
+        if constexpr (CUT) {
+          if (row0 + lane < p.Sq) {
+            const int64_t prow = (static_cast<int64_t>(w.slice) * p.B * p.Hq + w.bh) * p.Sq + row0 + lane;
 #pragma unroll
-          for (int u = 0; u < 8; ++u) ptx::st_global_v4(p.part_o + prow * D + col * 32 + u * 4, make_uint4(v[u * 4], v[u * 4 + 1], v[u * 4 + 2], v[u * 4 + 3]));
-          if (col == 0) *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(st.m, st.l);
-        } else if (qi < p.Sq) {
+            for (int u = 0; u < 8; ++u) ptx::st_global_v4(p.part_o + prow * D + col * 32 + u * 4, make_uint4(v[u * 4], v[u * 4 + 1], v[u * 4 + 2], v[u * 4 + 3]));
+            if (col == 0) *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(st.m, st.l);
+          }
+        } else {
+          // 64 columns at a time through shared memory (its 128-byte swizzle is the map's) and out by one copy: stores of a row a thread
+          // took 2.5 us of every piece (1 x 32 / 8 x 8192, window 1024: 150 us, without any stores 136)
+          const uint32_t at = ptx::smem_u32(sout + warp * 4096) + static_cast<uint32_t>(lane * 128);
+          if ((col & 1) == 0) {
+            if (lane == 0) ptx::bulk_wait_group_read<0>();  // the copy before has read the place
+            __syncwarp();
+          }
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             uint32_t x[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               x[e] = pack16<FMT>(__uint_as_float(v[u * 8 + 2 * e]) * inv, __uint_as_float(v[u * 8 + 2 * e + 1]) * inv);
-            ptx::st_global_v4(orow + col * 64 + u * 16, make_uint4(x[0], x[1], x[2], x[3]));
+            ptx::st_shared_v4(at + static_cast<uint32_t>(((((col & 1) * 4 + u) ^ (lane & 7)) * 16)), make_uint4(x[0], x[1], x[2], x[3]));
+          }
+          if ((col & 1) == 1) {
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && row0 < p.Sq) {
+              ptx::tma_store_3d(&p.tm_o, ptx::smem_u32(sout + warp * 4096), (col >> 1) * 64, row0, w.bh);
+              ptx::bulk_commit_group();
+            }
           }
         }
       }
@@ -437,6 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       ptx::tcgen05_fence_before();
     }
     if (!ok && lane == 0) { fail(p, 3u, t); *abort_flag = 1; }
+    if (!CUT && lane == 0) ptx::bulk_wait_group_all();      // what is on its way out has been read and written
   }
 
   ptx::tcgen05_fence_before();
@@ -569,10 +567,10 @@ extern "C" int catcoc_window_attention(const void* q, const void* k, const void*
   int rc = encode_bsd(&p.tm_q, q, dt, static_cast<int64_t>(B) * Hq, Sq, D);
   if (rc == 0) rc = encode_bsd(&p.tm_k, k, dt, static_cast<int64_t>(B) * Hk, Sk, D);
   if (rc == 0) rc = encode_bsd(&p.tm_v, v, dt, static_cast<int64_t>(B) * Hk, Sk, D);
-  if (rc != 0) return rc;
   const int64_t rows = static_cast<int64_t>(B) * Hq * Sq, works = static_cast<int64_t>(B) * Hq * d.tiles;
   if (works > (1 << 30)) { set_error("flash_attention: too many query tiles"); return CATCOC_E_TOO_LARGE; }
-  p.out = out;
+  if (rc == 0) rc = encode_rows(&p.tm_o, out, dt, static_cast<int64_t>(B) * Hq, Sq, D, 32);
+  if (rc != 0) return rc;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = workspace != nullptr ? p.part_o + d.slices * rows * D : nullptr;
   p.B = B; p.Hq = Hq; p.Hk = Hk; p.Sq = Sq; p.Sk = Sk; p.pos = pos;
@@ -594,7 +592,7 @@ extern "C" int catcoc_window_attention(const void* q, const void* k, const void*
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   const dim3 grid(static_cast<unsigned>(std::min<int64_t>(works * d.slices, catcoc_num_sms(device))));
   const int db = D / 64, slots = D == 128 ? 4 : 8;
-  const size_t smem = static_cast<size_t>(window::kTiles * db + slots * db) * window::kBlockBytes + sizeof(window::Bars) + 1024 + 64;
+  const size_t smem = static_cast<size_t>(window::kTiles * db + slots * db) * window::kBlockBytes + window::kOutBytes + sizeof(window::Bars) + 1024;
   auto launch = [&](auto kernel) -> int {
     CATCOC_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     CATCOC_CUDA_OK(launch_overlapped(kernel, grid, dim3(window::kThreads), smem, stream, p));
