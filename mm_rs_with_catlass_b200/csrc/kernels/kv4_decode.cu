@@ -1,21 +1,28 @@
 // Attention of a decode step over the paged 4-bit cache (layout: catcoc/kv4.h).
 //
-// The query heads that share a KV head, and the new tokens of a sequence, are the rows of one unit; every code is read once for all
-// of them. The blocks of all units form one list, by the lengths on the device, that is cut into equal runs over the CTAs; pieces
-// of a unit that lies in several runs are merged by a second kernel, and a third one adds the probabilities to the caller's sums.
+// The query heads that share a KV head, and the new tokens of a sequence, are the rows of a unit (up to 16 of them); every code is read
+// once for all of them. The blocks of all units form one list, by the lengths on the device, that is cut into equal runs over the CTAs;
+// pieces of a unit that lies in several runs are merged by a second kernel, and a third one adds the probabilities to the caller's sums.
 //
-// The four warps of a CTA take half blocks (32 tokens) in turn, each with bulk copies, a softmax and an O of its own; they meet at the end of
-// a unit. No warp waits for another one's copies, and none only copies.
+//   warps 0..3  32 tokens of a stage (two blocks) each, with a softmax and an O of their own; merged at the end of a unit
+//   warp 4      producer: one bulk copy a block (72 D bytes) into a ring of stages
 //
 // Both products run on codes, without their values: with scales and zeros constant over a group g of channels,
 //   q . k_j = sum_g s_jg (sum_c q_c code_jc) + z_jg (sum_c q_c),   o_c = sum_j (p_j s_jg) code_jc + sum_j p_j z_jg,
-// so that a code costs a mask (0.6 instructions, the values 4 tokens at a time 0.75): four bits at the bottom of a half are the
-// subnormal code * 2^-24, those above them code * 2^-20, both exact operands. The 16 between them goes into q and into the result.
-// q is brought into the range of a half by a power of two per row, p s by one per group that follows the largest scale, so
-// that the only rounding in front of the accumulators is that of p s to 11 bits.
+// so that a code costs a mask (five instructions for eight codes of K, six for V's): four bits at the bottom of a half are the subnormal
+// code * 2^-24, those above them code * 2^-20, both exact operands. The 16 between them goes into q and into the result. q is brought into
+// the range of a half by a power of two per row, p s by one per group that follows the largest scale, so that the only rounding in
+// front of the accumulators is that of p s to 11 bits.
 //
-// S^T = K q^T has the tokens as rows; its accumulator, scaled, rounded and transposed by movmatrix, is the second operand of
-// O^T += V^T (p s). Tokens fill the 16 rows of an instruction where query rows would fill a part of them.
+// S^T = K q^T has the tokens as rows of mma.m16n8k16; its accumulator, scaled, rounded and transposed by movmatrix, is the second operand of
+// O^T += V^T (p s). With up to four rows over two groups of channels (PAIR) the eight columns are four rows of each group, so that no lane
+// works on columns that do not exist.
+//
+// Bound by instruction issue. The products are a stream of codes that have to become 16-bit operands, 43 a cycle and SM at the memory's rate;
+// in the registers they are operands as soon as they are masked. The tensor cores' own memory was built too and was slower (16 x 8 heads x
+// 4096 tokens, four rows, 75 MB): K into TMEM and V into shared memory as halves, scores a token a thread, tcgen05.mma for both products took
+// 37.6 us with four warps twice on an SM and 38.5 us with four teams of four warps and a fifth for issue and copies: a step of 128 tokens was a
+// chain of eight waits of 500 to 1900 cycles.
 #include <cuda_fp16.h>
 #include <algorithm>
 #include <cstring>
@@ -31,9 +38,11 @@
 namespace catcoc {
 namespace kv4 {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = 32 * kWarps;
+constexpr int kWarps = 4;                          // consumer warps
+constexpr int kThreads = 32 * (kWarps + 1), kWorkers = 32 * kWarps;
 constexpr int kTile = 16;                          // tokens of a matrix instruction
+constexpr int kSub = 2;                            // blocks of a stage
+constexpr int kItem = kSub * kPage / kWarps;       // tokens of a stage that a warp takes
 constexpr int kPShift = 5;                         // p s is held times 2^(5 - e), e: exponent of the largest scale; p <= 2^8, so below 2^14
 
 struct DecodeParams {
@@ -69,9 +78,14 @@ CATCOC_DEVICE Span span_of(int len, int q_len, int window, int sinks) {
     const int lo = len - q_len - window + 1;       // first key of the first new token's window
     s.first = lo > 0 ? lo / kPage : 0;
     s.sink = min((sinks + kPage - 1) / kPage, s.first);
-    if (s.sink < 0) s.sink = 0;
   }
   return s;
+}
+
+// Blocks of a CTA's run; stages take two, so runs of more than two are even
+CATCOC_DEVICE int blocks_per_run(int total, int ctas) {
+  const int per = (total + ctas - 1) / ctas;
+  return per > kSub ? (per + 1) & ~1 : per;
 }
 
 CATCOC_DEVICE void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -89,167 +103,171 @@ CATCOC_DEVICE uint32_t half2_of(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Tokens of an item, what a warp takes at once: half a block, so that short runs keep the warps busy too
-constexpr int kItem = 32;
-constexpr int kSubs = kPage / kItem;
-
-// A part of the run: blocks [i0, i1) of the n of a unit's list (Hk x chunks units a sequence)
-struct Part {
-  int b, unit, i0, i1, n;
-};
-// The next item of a warp and its part, which begins at `at` of the list
-struct Ahead {
-  Part part;
-  int at, item, more;
-};
-
-template <int D, int NT>
-struct Smem {
-  using L = Block<D>;
-  // an item: codes of K and of V, then their parameters
-  static constexpr int kCodes = kItem * L::kRow, kPars = kItem * L::kParRow;
-  static constexpr int kStageBytes = 2 * (kCodes + kPars);
-  static constexpr int kStages = 2;    // of every warp
-  alignas(128) uint8_t stage[kWarps][kStages][kStageBytes];
-  float o[kWarps][8 * NT][D + 4];      // (4: the lanes of a warp store to different banks)
-  float2 ml[kWarps][8 * NT];
-  uint64_t full[kWarps][kStages];
-  uint32_t abort_flag;
-  uint32_t failed[kWarps];
-  Ahead ahead[kWarps];
-  int seqs[1];                         // [B + 1] blocks of the sequences before, then [B] lengths
-};
-
 // Row of a matrix instruction -> token of the tile. Two tokens of a pair are swapped in every other pair, so that the rows that four
 // lanes read of V lie in both halves of the banks (K's stay free of conflicts).
 CATCOC_DEVICE int token_of(int row) { return row ^ ((row >> 1) & 1); }
 
-// D: head dimension, FMT: type of q and out, NT: query rows of a unit in eights, W: the scores are written for the weights
-template <int D, int FMT, int NT, bool W>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
+// A part of the run: blocks [i0, i1) of the n of a unit's list. The sequence's units (Hk x chunks of n blocks) begin at `base` of the list.
+struct Part {
+  int b, base, n, len;
+  int unit, i0, i1;
+};
+
+// NT: rows of a unit in eights; PAIR: four rows (D = 128)
+template <int D, int NT, bool PAIR>
+struct Geo {
+  static constexpr int G = Block<D>::kGroups;
+  static constexpr int kRows = PAIR ? 4 : 8 * NT;
+  static constexpr int kStages = D == 128 ? 3 : 5;
+  static constexpr int kCtas = NT == 1 ? 3 : 2;    // of an SM
+};
+template <int D, int NT, bool PAIR>
+struct Smem {
+  using Ge = Geo<D, NT, PAIR>;
+  alignas(128) uint8_t stage[Ge::kStages][kSub][Block<D>::kBytes];
+  float o[kWarps][Ge::kRows][D + 4];   // (4: the lanes of a warp store to different banks)
+  float2 ml[kWarps][Ge::kRows];
+  uint64_t full[Ge::kStages], empty[Ge::kStages];
+  uint32_t abort_flag, failed[kWarps];
+  int total;                           // blocks of the list
+  Part start;                          // the sequence in which the run begins
+};
+
+// D: head dimension, FMT: type of q and out, W: the scores are written for the weights
+template <int D, int FMT, int NT, bool PAIR, bool W>
+__global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
   using L = Block<D>;
-  using Sm = Smem<D, NT>;
-  constexpr int G = L::kGroups, kRowsU = 8 * NT;
+  using Ge = Geo<D, NT, PAIR>;
+  using Sm = Smem<D, NT, PAIR>;
+  static_assert(!PAIR || (NT == 1 && L::kGroups == 2));
+  constexpr int G = Ge::G, kRows = Ge::kRows;
+  constexpr int GL = PAIR ? 1 : G;               // groups of channels that a lane's columns stand for
   extern __shared__ uint8_t smem_raw[];
   Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
-  int* prefix = sm.seqs;
-  int* seq_lens = sm.seqs + p.B + 1;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile uint32_t* abort_flag = &sm.abort_flag;
+  const int per_seq = p.Hk * p.chunks;            // units of a sequence
+  auto span_at = [&](int len) { return span_of(len, p.q_len, p.window, p.sinks); };
 
-  if (lane == 0) {
-    for (int s = 0; s < Sm::kStages; ++s) ptx::mbar_init(&sm.full[warp][s], 1);
-    if (warp == 0) sm.abort_flag = 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < Ge::kStages; ++s) { ptx::mbar_init(&sm.full[s], 1); ptx::mbar_init(&sm.empty[s], kWarps); }
+    sm.abort_flag = 0;
     ptx::mbar_fence_init();
   }
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
-  // blocks of the sequences before each one
-  if (warp == 0) {
+  if (warp == kWarps) {
+    // the blocks of all sequences, and the sequence in which this CTA's run begins
     int sum = 0;
-    for (int base = 0; base < p.B; base += 32) {
-      const int b = base + lane;
-      int n = 0;
-      if (b < p.B) {
-        const int len = seq_len(p.lens, b, p.max_pages * kPage, p.status);
-        seq_lens[b] = len;
-        n = span_of(len, p.q_len, p.window, p.sinks).count();
-      }
+    for (int b = lane; b < p.B; b += 32) sum += span_at(seq_len(p.lens, b, p.max_pages * kPage, p.status)).count();
+    const int total = __reduce_add_sync(0xffffffffu, sum) * per_seq;
+    const int begin = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * blocks_per_run(total, static_cast<int>(gridDim.x)), static_cast<int64_t>(total)));
+    int behind = 0, start = 0, base = 0;
+    for (int chunk = 0; chunk < p.B; chunk += 32) {
+      const int b = chunk + lane, mine = b < p.B ? span_at(seq_len(p.lens, b, p.max_pages * kPage, p.status)).count() : 0;
+      int n = mine;
 #pragma unroll
       for (int o = 1; o < 32; o *= 2) {
         const int y = __shfl_up_sync(0xffffffffu, n, o);
         if (lane >= o) n += y;
       }
-      if (b < p.B) prefix[b + 1] = sum + n;
-      sum += __shfl_sync(0xffffffffu, n, 31);
+      n += behind;
+      if (blockIdx.x == 0 && b < p.B) p.prefix[b + 1] = n;
+      const uint32_t hit = __ballot_sync(0xffffffffu, b < p.B && (n - mine) * per_seq <= begin && begin < n * per_seq);
+      if (hit != 0u) {
+        start = chunk + __ffs(hit) - 1;
+        base = __shfl_sync(0xffffffffu, (n - mine) * per_seq, __ffs(hit) - 1);
+        if (blockIdx.x != 0) break;
+      }
+      behind = __shfl_sync(0xffffffffu, n, 31);
     }
-    if (lane == 0) prefix[0] = 0;
-    __syncwarp();
-    if (blockIdx.x == 0)
-      for (int b = lane; b <= p.B; b += 32) p.prefix[b] = prefix[b];
+    if (lane == 0) {
+      if (blockIdx.x == 0) p.prefix[0] = 0;
+      const int len = seq_len(p.lens, start, p.max_pages * kPage, p.status);
+      sm.total = total;
+      sm.start = Part{start, base, span_at(len).count(), len, 0, 0, 0};
+    }
   }
   __syncthreads();
-  const int per_seq = p.Hk * p.chunks;                            // units of a sequence
-  const int total = prefix[p.B] * per_seq;
-  const int per = (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
-  const int begin = min(total, static_cast<int>(blockIdx.x) * per), end = min(total, begin + per);
-  // the part of the run that begins at list position `at`, in sequence `b` or behind it
-  auto part_at = [&](int at, int b) {
-    while (prefix[b + 1] * per_seq <= at) ++b;
-    const int n = prefix[b + 1] - prefix[b], in_seq = at - prefix[b] * per_seq, unit = in_seq / n, i0 = in_seq - unit * n;
-    return Part{b, unit, i0, min(n, i0 + end - at), n};
-  };
-  int b0 = 0;                                                     // the last sequence that begins at or before `begin`
-  for (int hi = p.B; hi - b0 > 1;) {
-    const int mid = (b0 + hi) >> 1;
-    if (prefix[mid] * per_seq <= begin) b0 = mid; else hi = mid;
-  }
-
-  // ------------------------------ copies ------------------------------
-  // A warp fetches what it will work on, two items ahead and across parts. Item x of a part goes to warp x % 4. The name
-  // of an item's block is read when the item before it is requested.
-  // What it is at lies in shared memory: it is needed once an item, and the registers are short. (The name does not: a store
-  // would wait for it.)
-  Ahead& ahead = sm.ahead[warp];
-  int requested = 0, ahead_page = -1;
-  auto look = [&](Ahead a) {                                      // from a.at, a.item on to the next item of this warp
-    while (!(a.more && a.item < (a.part.i1 - a.part.i0) * kSubs)) {
-      if (a.more) a.at += a.part.i1 - a.part.i0;
-      const int b = a.more ? a.part.b : b0;
-      a.more = a.at < end;
-      if (!a.more) break;
-      a.part = part_at(a.at, b);
-      a.item = warp;
+  const int total = sm.total;
+  const int per = blocks_per_run(total, static_cast<int>(gridDim.x));
+  const int begin = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * per, static_cast<int64_t>(total))), end = min(total, begin + per);
+  // the part of the run that begins at list position `at`, in the sequence of `s` or behind it
+  auto part_at = [&](int at, Part s) {
+    while (s.base + s.n * per_seq <= at) {
+      s.base += s.n * per_seq;
+      ++s.b;
+      s.len = seq_len(p.lens, s.b, p.max_pages * kPage, p.status);
+      s.n = span_at(s.len).count();
     }
-    if (a.more)
-      ahead_page = p.table[static_cast<int64_t>(a.part.b) * p.max_pages + span_of(seq_lens[a.part.b], p.q_len, p.window, p.sinks).block(a.part.i0 + a.item / kSubs)];
-    __syncwarp();
-    if (lane == 0) ahead = a;
-    __syncwarp();
+    s.unit = (at - s.base) / s.n;
+    s.i0 = at - s.base - s.unit * s.n;
+    s.i1 = min(s.n, s.i0 + end - at);
+    return s;
   };
-  auto request = [&] {
-    Ahead a = ahead;
-    if (!a.more) return;
-    const int s = requested % Sm::kStages;
-    uint64_t* bar = &sm.full[warp][s];
-    if (lane == 0) {
-      if (static_cast<uint32_t>(ahead_page) < static_cast<uint32_t>(p.pages)) {
-        const uint8_t* src = p.cache + (static_cast<int64_t>(ahead_page) * p.Hk + a.part.unit / p.chunks) * L::kBytes;
-        const int sub = a.item % kSubs;
-        uint8_t* dst = sm.stage[warp][s];
-        ptx::mbar_expect_tx(bar, Sm::kStageBytes);
+  uint32_t step = 0;                              // stages so far
+  Part part = sm.start;
+
+  if (warp == kWarps) {
+    // ------------------------------ producer ------------------------------
+    bool ok = true;
+    for (int at = begin; ok && at < end; at += part.i1 - part.i0) {
+      part = part_at(at, part);
+      const Span span = span_at(part.len);
+      const int hk = part.unit / p.chunks;
+      int ids = -1;
+      for (int i = part.i0; i < part.i1; i += kSub, ++step) {
+        // the names of 32 blocks at a time, so that no copy waits for its own
+        const int k = (i - part.i0) & 31;
+        if (k == 0) ids = i + lane < part.i1 ? page_of(p.table, static_cast<int64_t>(part.b) * p.max_pages, span.block(i + lane), p.pages, p.status) : -1;
+        const uint32_t stage = step % Ge::kStages;
+        ok = ptx::mbar_wait(&sm.empty[stage], ((step / Ge::kStages) & 1u) ^ 1u, p.timeout_ns, abort_flag);
+        if (!ok) break;
+        int page[kSub], found = 0;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          ptx::bulk_load_1d(dst + half * Sm::kCodes, src + half * L::kHalf + sub * Sm::kCodes, Sm::kCodes, bar);
-          ptx::bulk_load_1d(dst + 2 * Sm::kCodes + half * Sm::kPars, src + half * L::kHalf + L::kPar + sub * Sm::kPars, Sm::kPars, bar);
+        for (int s = 0; s < kSub; ++s) {
+          page[s] = __shfl_sync(0xffffffffu, ids, k + s);
+          found += page[s] >= 0;
         }
-      } else {
-        note(p.status, kErrPage, ahead_page, p.pages);                // what the stage held stands in for the block
-        ptx::mbar_arrive(bar);
+        if (lane == 0) {
+          // (a block that is not in the cache was noted: what the stage held stands in for it)
+          if (found == 0) ptx::mbar_arrive(&sm.full[stage]);
+          else ptx::mbar_expect_tx(&sm.full[stage], static_cast<uint32_t>(found * L::kBytes));
+#pragma unroll
+          for (int s = 0; s < kSub; ++s)
+            if (page[s] >= 0)
+              ptx::bulk_load_1d(sm.stage[stage][s], p.cache + (static_cast<int64_t>(page[s]) * p.Hk + hk) * L::kBytes, L::kBytes, &sm.full[stage]);
+        }
+        __syncwarp();
       }
     }
-    ++requested;
-    a.item += kWarps;
-    look(a);
-  };
-  look(Ahead{{}, begin, 0, 0});
-  for (int s = 0; s < Sm::kStages; ++s) request();
+    if (!ok || *abort_flag != 0) {
+      // the run was given up: the copies that are still on their way land before the block's memory is handed on
+      if (lane == 0) *abort_flag = 1;
+      volatile uint32_t never = 0;
+      for (uint32_t i = step > Ge::kStages ? step - Ge::kStages : 0; i < step; ++i)
+        ptx::mbar_wait(&sm.full[i % Ge::kStages], (i / Ge::kStages) & 1u, 100000000ull, &never);
+    }
+    return;
+  }
 
   // ------------------------------ products and softmax ------------------------------
-  int taken = 0;
+  const int g8 = lane >> 2, t4 = lane & 3;
+  const int own = PAIR ? t4 >> 1 : 0;             // PAIR: the group of this lane's columns
+  const int sub = warp / (kWarps / kSub), token0 = (warp % (kWarps / kSub)) * kItem;   // this warp's block of a stage, and its tokens there
+  auto row_of = [&](int nt, int c) { return PAIR ? 2 * (t4 & 1) + c : nt * 8 + 2 * t4 + c; };   // row of the unit that a lane's column stands for
   bool ok = true;
-  Part part{};
   for (int at = begin; at < end && ok; at += part.i1 - part.i0) {
-    part = part_at(at, at > begin ? part.b : b0);
-    const int b = part.b, len = seq_lens[b];
-    const Span span = span_of(len, p.q_len, p.window, p.sinks);
-    const int hk = part.unit / p.chunks, row0 = (part.unit - hk * p.chunks) * kRowsU;   // first row of the unit among the R of its head
-    // q as the second operand of S^T: row g8 of every eight, the channels of this lane's words; b0, b1 of every step
+    part = part_at(at, part);
+    const int b = part.b, len = part.len;
+    const Span span = span_at(len);
+    const int hk = part.unit / p.chunks, row0 = (part.unit - hk * p.chunks) * kRows;   // first row of the unit among the R of its head
+    // q as the second operand of S^T: column g8 of every eight, the channels of this lane's words; b0, b1 of every step
     uint32_t qf[NT][2 * G][4];
-    float qscale[NT][2], qsum[NT][G][2];              // of the rows of this lane's columns, 2 t4 and 2 t4 + 1: score = qscale * raw
+    float qscale[NT][2], qsum[NT][GL][2];             // of the rows of this lane's columns: score = qscale * raw score
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = row0 + nt * 8 + g8;
+      const int r = row0 + (PAIR ? g8 & 3 : nt * 8 + g8);
       const int tok = r / p.group;
       const uint16_t* src = static_cast<const uint16_t*>(p.q) + ((static_cast<int64_t>(b) * p.q_len + tok) * p.Hq + hk * p.group + (r - tok * p.group)) * D;
       float x[2 * G][8], mx = 0.0f, sum[G] = {};
@@ -274,10 +292,11 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
 #pragma unroll
       for (int i = 0; i < 2 * G; ++i) {
         // steps of a word: its bits 0-3, 4-7 (and 16-19, 20-23), then 8-11, 12-15 (and 24-27, 28-31)
-        qf[nt][i][0] = half2_of(x[i][0] * f, x[i][4] * f);
-        qf[nt][i][1] = half2_of(x[i][1] * f * 0.0625f, x[i][5] * f * 0.0625f);
-        qf[nt][i][2] = half2_of(x[i][2] * f, x[i][6] * f);
-        qf[nt][i][3] = half2_of(x[i][3] * f * 0.0625f, x[i][7] * f * 0.0625f);
+        const float h = PAIR && i % G != (g8 >> 2) ? 0.0f : f, h16 = h * 0.0625f;   // PAIR: a column knows the channels of its group alone
+        qf[nt][i][0] = half2_of(x[i][0] * h, x[i][4] * h);
+        qf[nt][i][1] = half2_of(x[i][1] * h16, x[i][5] * h16);
+        qf[nt][i][2] = half2_of(x[i][2] * h, x[i][6] * h);
+        qf[nt][i][3] = half2_of(x[i][3] * h16, x[i][7] * h16);
       }
       const float back = p.scale_log2 * 16777216.0f / f;
 #pragma unroll
@@ -286,59 +305,60 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
         sum[g] += __shfl_xor_sync(0xffffffffu, sum[g], 2);
         sum[g] *= f * (1.0f / 16777216.0f);           // in the unit of the products of codes
       }
+      if constexpr (PAIR) sum[0] = g8 < 4 ? sum[0] : sum[1];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int from = (2 * t4 + c) * 4;
+        const int from = (2 * t4 + c) * 4;            // a lane of that column
         qscale[nt][c] = __shfl_sync(0xffffffffu, back, from);
 #pragma unroll
-        for (int g = 0; g < G; ++g) qsum[nt][g][c] = __shfl_sync(0xffffffffu, sum[g], from);
+        for (int g = 0; g < GL; ++g) qsum[nt][g][c] = __shfl_sync(0xffffffffu, sum[g], from);
       }
     }
     // m: largest raw score, as far as it is followed; m_neg: minus its score; limit: raw score from which on it moves
-    float o[NT][G][4][4] = {}, m[NT][2], m_neg[NT][2], limit[NT][2], l[NT][2] = {}, zsum[NT][G][2] = {};
-    int e_ref[G];                                     // exponent field that the scales of V are held against
-    float vscale[G];                                  // 2^(kPShift + 127 - e_ref)
+    float o[NT][G][4][4] = {}, m[NT][2], m_neg[NT][2], limit[NT][2], l[NT][2] = {}, zsum[NT][GL][2] = {};
+    uint32_t e_ref[GL];                               // exponent field that the scales of V are held against
+    float vscale[GL];                                 // 2^(kPShift + 127 - e_ref)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) { m[nt][c] = limit[nt][c] = -INFINITY; m_neg[nt][c] = 0.0f; }
 #pragma unroll
-    for (int g = 0; g < G; ++g) { e_ref[g] = 8; vscale[g] = __uint_as_float((254u + kPShift - 8u) << 23); }
+    for (int g = 0; g < GL; ++g) { e_ref[g] = 8; vscale[g] = __uint_as_float((254u + kPShift - 8u) << 23); }
     const int pos_lo = len - p.q_len, pos_hi = len - 1;
 
-    // TILES tiles from token `t0` of the stage on. ALL: every row sees every key of them.
-    auto tiles = [&](auto all_c, auto count_c, const uint8_t* st, int t0, int key0) {
+    // TILES tiles from token `t0` of a block on. ALL: every row sees every key of them.
+    auto tiles = [&](auto all_c, auto count_c, const uint8_t* block, int t0, int key0) {
       constexpr bool ALL = decltype(all_c)::value;
       constexpr int TILES = decltype(count_c)::value;
-      const uint8_t *kc = st + t0 * L::kRow, *vc = kc + Sm::kCodes, *kp = st + 2 * Sm::kCodes + t0 * L::kParRow, *vp = kp + Sm::kPars;
+      const uint8_t *kc = block + t0 * L::kRow, *vc = kc + L::kHalf, *kp = block + L::kPar + t0 * L::kParRow, *vp = kp + L::kHalf;
       float s[TILES][NT][4];
-      uint32_t vpar[TILES][2][G];
+      uint32_t vpar[TILES][2][GL];
       const int tk = token_of(g8);
 #pragma unroll
       for (int i = 0; i < TILES; ++i) {
-        // S^T: rows g8 and g8 + 8 are tokens, channels by t4; one accumulator per group
-        uint32_t ka[2 * G], kb[2 * G], par[2][G];
-        const uint8_t* at = kc + (i * kTile + tk) * L::kRow + t4 * 8 * G;
+        // S^T: rows g8 and g8 + 8 are tokens, channels by t4
+        uint32_t ka[2 * G], kb[2 * G], par[2][GL];
+        const uint8_t* from = kc + (i * kTile + tk) * L::kRow + t4 * 8 * G;
         if constexpr (G == 2) {
-          const uint4 a = *reinterpret_cast<const uint4*>(at), c = *reinterpret_cast<const uint4*>(at + 8 * L::kRow);
-          ka[0] = a.x; ka[1] = a.y; ka[2] = a.z; ka[3] = a.w;
-          kb[0] = c.x; kb[1] = c.y; kb[2] = c.z; kb[3] = c.w;
+          const uint4 x = *reinterpret_cast<const uint4*>(from), y = *reinterpret_cast<const uint4*>(from + 8 * L::kRow);
+          ka[0] = x.x; ka[1] = x.y; ka[2] = x.z; ka[3] = x.w;
+          kb[0] = y.x; kb[1] = y.y; kb[2] = y.z; kb[3] = y.w;
         } else {
-          const uint2 a = *reinterpret_cast<const uint2*>(at), c = *reinterpret_cast<const uint2*>(at + 8 * L::kRow);
-          ka[0] = a.x; ka[1] = a.y;
-          kb[0] = c.x; kb[1] = c.y;
+          const uint2 x = *reinterpret_cast<const uint2*>(from), y = *reinterpret_cast<const uint2*>(from + 8 * L::kRow);
+          ka[0] = x.x; ka[1] = x.y;
+          kb[0] = y.x; kb[1] = y.y;
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const int off = (i * kTile + tk + 8 * u) * L::kParRow;
-          if constexpr (G == 2) {
-            const uint2 a = *reinterpret_cast<const uint2*>(kp + off), c = *reinterpret_cast<const uint2*>(vp + off);
-            par[u][0] = a.x; par[u][1] = a.y; vpar[i][u][0] = c.x; vpar[i][u][1] = c.y;
+          const int off = (i * kTile + tk + 8 * u) * L::kParRow + own * 4;
+          if constexpr (GL == 2) {
+            const uint2 x = *reinterpret_cast<const uint2*>(kp + off), y = *reinterpret_cast<const uint2*>(vp + off);
+            par[u][0] = x.x; par[u][1] = x.y; vpar[i][u][0] = y.x; vpar[i][u][1] = y.y;
           } else {
             par[u][0] = *reinterpret_cast<const uint32_t*>(kp + off); vpar[i][u][0] = *reinterpret_cast<const uint32_t*>(vp + off);
           }
         }
-        float acc[NT][G][4] = {};
+        float acc[NT][G][4] = {};                     // (PAIR: the groups' columns differ, their sum is both)
 #pragma unroll
         for (int w = 0; w < 2 * G; ++w) {
           const uint32_t a8 = ka[w] >> 8, b8 = kb[w] >> 8;
@@ -348,17 +368,22 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
             mma_f16(acc[nt][w % G], a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u, qf[nt][w][2], qf[nt][w][3]);
           }
         }
-        // raw scores of tokens g8 ([0], [1]) and g8 + 8 ([2], [3]), columns 2 t4 and 2 t4 + 1
+        // raw scores of tokens g8 ([0], [1]) and g8 + 8 ([2], [3]), this lane's two columns
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int u = e >> 1, c = e & 1;
             float a = bf16_hi(par[u][0]) * qsum[nt][0][c];
+            if constexpr (PAIR) {
+              a = fmaf(bf16_lo(par[u][0]), acc[nt][0][e] + acc[nt][G - 1][e], a);
+              a += __shfl_xor_sync(0xffffffffu, a, 2);
+            } else {
 #pragma unroll
-            for (int g = 1; g < G; ++g) a = fmaf(bf16_hi(par[u][g]), qsum[nt][g][c], a);
+              for (int g = 1; g < G; ++g) a = fmaf(bf16_hi(par[u][g]), qsum[nt][g][c], a);
 #pragma unroll
-            for (int g = 0; g < G; ++g) a = fmaf(bf16_lo(par[u][g]), acc[nt][g][e], a);
+              for (int g = 0; g < G; ++g) a = fmaf(bf16_lo(par[u][g]), acc[nt][g][e], a);
+            }
             s[i][nt][e] = a;
           }
         if constexpr (!ALL) {
@@ -368,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int r = row0 + nt * 8 + 2 * t4 + (e & 1);
+              const int r = row0 + row_of(nt, e & 1);
               const bool v = r < p.R && sees(pos_lo + r / p.group, key0 + i * kTile + tk + 8 * (e >> 1), p.window, p.sinks);
               if (!v) s[i][nt][e] = -INFINITY;
               seen[e >> 1] |= v;
@@ -376,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
 #pragma unroll
           for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int g = 0; g < G; ++g)
+            for (int g = 0; g < GL; ++g)
               if (!seen[u]) vpar[i][u][g] = 0u;
         }
         if constexpr (W) {
@@ -385,8 +410,8 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              const int r = row0 + nt * 8 + 2 * t4 + c;
-              if (r < p.R) {
+              const int r = row0 + row_of(nt, c);
+              if (r < p.R && own == 0) {
                 dst[static_cast<int64_t>(r) * p.S] = s[i][nt][c] * qscale[nt][c];
                 dst[static_cast<int64_t>(r) * p.S + 8] = s[i][nt][2 + c] * qscale[nt][c];
               }
@@ -394,18 +419,17 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
         }
       }
       // the references: m moves when a score exceeds its own by more than 8, e_ref when a scale is past twice its power
-      float ps[TILES][G][2], top = 0.0f;
-      bool move = false;
+      float ps[TILES][GL][2], top = 0.0f;
 #pragma unroll
       for (int i = 0; i < TILES; ++i)
 #pragma unroll
-        for (int g = 0; g < G; ++g)
+        for (int g = 0; g < GL; ++g)
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             ps[i][g][u] = bf16_lo(vpar[i][u][g]) * vscale[g];
             top = fmaxf(top, ps[i][g][u]);
           }
-      move = top >= static_cast<float>(2 << kPShift);
+      bool move = top >= static_cast<float>(2 << kPShift);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -416,22 +440,24 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
           move |= x > limit[nt][c];
         }
       if (__any_sync(0xffffffffu, move)) {
-        float beta[G];
+        float beta[GL];
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
+        for (int g = 0; g < GL; ++g) {
           // (scales are not negative; one that is no number, or infinite, sets no reference)
-          uint32_t ex = 0;
+          uint32_t e_new = e_ref[g];
 #pragma unroll
           for (int i = 0; i < TILES; ++i)
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               const uint32_t x = (vpar[i][u][g] >> 7) & 0xffu;
-              ex = max(ex, x == 255u ? 0u : x);
+              e_new = max(e_new, x == 255u ? 0u : x);
             }
-          const int e_new = max(e_ref[g], static_cast<int>(__reduce_max_sync(0xffffffffu, ex)));
-          beta[g] = e_new - e_ref[g] > 126 ? 0.0f : __uint_as_float(static_cast<uint32_t>(127 + e_ref[g] - e_new) << 23);
+#pragma unroll
+          for (int d = 1; d < 32; d *= 2)
+            if (d != 2) e_new = max(e_new, __shfl_xor_sync(0xffffffffu, e_new, d));   // (lanes t4 and t4 ^ 2 may stand for two groups)
+          beta[g] = e_new - e_ref[g] > 126u ? 0.0f : __uint_as_float((127u + e_ref[g] - e_new) << 23);
           e_ref[g] = e_new;
-          vscale[g] = __uint_as_float((254u + kPShift - static_cast<uint32_t>(e_new)) << 23);
+          vscale[g] = __uint_as_float((254u + kPShift - e_new) << 23);
 #pragma unroll
           for (int i = 0; i < TILES; ++i)
 #pragma unroll
@@ -453,19 +479,19 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
             limit[nt][c] = mn + attn::kLazyRescale / qscale[nt][c];
             l[nt][c] *= alpha;
 #pragma unroll
-            for (int g = 0; g < G; ++g) {
-              zsum[nt][g][c] *= alpha;
+            for (int g = 0; g < GL; ++g) zsum[nt][g][c] *= alpha;
+#pragma unroll
+            for (int g = 0; g < G; ++g)
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
-                o[nt][g][k][c] *= alpha * beta[g];
-                o[nt][g][k][2 + c] *= alpha * beta[g];
+                o[nt][g][k][c] *= alpha * beta[g % GL];
+                o[nt][g][k][2 + c] *= alpha * beta[g % GL];
               }
-            }
           }
       }
 #pragma unroll
       for (int i = 0; i < TILES; ++i) {
-        uint32_t pb[NT][G][2];
+        uint32_t pb[NT][GL][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float pr[4];
@@ -475,7 +501,7 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
             l[nt][e & 1] += pr[e];
           }
 #pragma unroll
-          for (int g = 0; g < G; ++g) {
+          for (int g = 0; g < GL; ++g) {
             float w[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -492,9 +518,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
         uint32_t vw[4][G];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-          const uint8_t* at = vc + (i * kTile + token_of(2 * t4 + (u & 1)) + 8 * (u >> 1)) * L::kRow + g8 * 4 * G;
-          if constexpr (G == 2) { const uint2 x = *reinterpret_cast<const uint2*>(at); vw[u][0] = x.x; vw[u][1] = x.y; }
-          else vw[u][0] = *reinterpret_cast<const uint32_t*>(at);
+          const uint8_t* from = vc + (i * kTile + token_of(2 * t4 + (u & 1)) + 8 * (u >> 1)) * L::kRow + g8 * 4 * G;
+          if constexpr (G == 2) { const uint2 x = *reinterpret_cast<const uint2*>(from); vw[u][0] = x.x; vw[u][1] = x.y; }
+          else vw[u][0] = *reinterpret_cast<const uint32_t*>(from);
         }
 #pragma unroll
         for (int g = 0; g < G; ++g)
@@ -504,37 +530,39 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
             const uint32_t x8 = x >> 8, y8 = y >> 8;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma_f16(o[nt][g][2 * hw], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, pb[nt][g][0], pb[nt][g][1]);
-              mma_f16(o[nt][g][2 * hw + 1], x8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u, pb[nt][g][0], pb[nt][g][1]);
+              mma_f16(o[nt][g][2 * hw], x & 0x000f000fu, x & 0x00f000f0u, y & 0x000f000fu, y & 0x00f000f0u, pb[nt][g % GL][0], pb[nt][g % GL][1]);
+              mma_f16(o[nt][g][2 * hw + 1], x8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u, pb[nt][g % GL][0], pb[nt][g % GL][1]);
             }
           }
       }
     };
 
-    for (int item = warp; item < (part.i1 - part.i0) * kSubs; item += kWarps) {
-      const int st = taken % Sm::kStages;
-      ok = ptx::mbar_wait(&sm.full[warp][st], static_cast<uint32_t>(taken / Sm::kStages) & 1u, p.timeout_ns, abort_flag);
+#pragma unroll 1
+    for (int i = part.i0; i < part.i1; i += kSub, ++step) {
+      const uint32_t stage = step % Ge::kStages;
+      ok = ptx::mbar_wait(&sm.full[stage], (step / Ge::kStages) & 1u, p.timeout_ns, abort_flag);
       if (!ok) break;
-      ++taken;
-      const int key0 = span.block(part.i0 + item / kSubs) * kPage + (item % kSubs) * kItem;
-      const uint8_t* stage = sm.stage[warp][st];
-      if (key0 + kItem - 1 <= pos_lo && (p.window == 0 || pos_hi - key0 < p.window || key0 + kItem <= p.sinks)) {
-        if constexpr (NT == 1) {
-          tiles(std::true_type{}, std::integral_constant<int, 2>{}, stage, 0, key0);
+      if (i + sub < part.i1) {
+        const int key0 = span.block(i + sub) * kPage + token0;
+        const uint8_t* block = sm.stage[stage][sub];
+        if (key0 + kItem - 1 <= pos_lo && (p.window == 0 || pos_hi - key0 < p.window || key0 + kItem <= p.sinks)) {
+          if constexpr (NT == 1) {
+            tiles(std::true_type{}, std::integral_constant<int, kItem / kTile>{}, block, token0, key0);
+          } else {
+#pragma unroll 1
+            for (int t = 0; t < kItem; t += kTile) tiles(std::true_type{}, std::integral_constant<int, 1>{}, block, token0 + t, key0 + t);
+          }
         } else {
 #pragma unroll 1
-          for (int t = 0; t < kItem; t += kTile) tiles(std::true_type{}, std::integral_constant<int, 1>{}, stage, t, key0 + t);
-        }
-      } else {
-#pragma unroll 1
-        for (int t = 0; t < kItem; t += kTile) {
-          const int k0 = key0 + t;
-          if (k0 <= pos_hi && (p.window == 0 || pos_lo - (k0 + kTile - 1) < p.window || k0 < p.sinks))
-            tiles(std::false_type{}, std::integral_constant<int, 1>{}, stage, t, k0);
+          for (int t = 0; t < kItem; t += kTile) {
+            const int k0 = key0 + t;
+            if (k0 <= pos_hi && (p.window == 0 || pos_lo - (k0 + kTile - 1) < p.window || k0 < p.sinks))
+              tiles(std::false_type{}, std::integral_constant<int, 1>{}, block, token0 + t, k0);
+          }
         }
       }
       __syncwarp();
-      request();                                       // into the stage that was just read
+      if (lane == 0) ptx::mbar_arrive(&sm.empty[stage]);
     }
 
     // the four warps' pieces of the unit: every one leaves its row, weighed against the largest maximum
@@ -546,49 +574,51 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
         for (int d = 4; d < 32; d *= 2) {
           l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], d);
 #pragma unroll
-          for (int g = 0; g < G; ++g) zsum[nt][g][c] += __shfl_xor_sync(0xffffffffu, zsum[nt][g][c], d);
+          for (int g = 0; g < GL; ++g) zsum[nt][g][c] += __shfl_xor_sync(0xffffffffu, zsum[nt][g][c], d);
         }
         // (from here on m is a score)
         m[nt][c] = m[nt][c] == -INFINITY ? -INFINITY : -m_neg[nt][c];
-        if (g8 == 0) sm.ml[warp][nt * 8 + 2 * t4 + c] = make_float2(m[nt][c], l[nt][c]);
+        if (g8 == 0 && own == 0) sm.ml[warp][row_of(nt, c)] = make_float2(m[nt][c], l[nt][c]);
       }
     if (!ok && lane == 0) *abort_flag = 1;
     if (lane == 0) sm.failed[warp] = ok ? 0u : 1u;
     // (every warp walks the same parts and takes all barriers, also after a failed wait; all leave together)
-    __syncthreads();
+    ptx::named_bar_sync(1, kWorkers);
     ok = (sm.failed[0] | sm.failed[1] | sm.failed[2] | sm.failed[3]) == 0u;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int r = nt * 8 + 2 * t4 + c;
+        const int r = row_of(nt, c);
         float mt = sm.ml[0][r].x;
 #pragma unroll
         for (int w = 1; w < kWarps; ++w) mt = fmaxf(mt, sm.ml[w][r].x);
         const float a = m[nt][c] == -INFINITY ? 0.0f : ptx::ex2_approx(m[nt][c] - mt);
 #pragma unroll
-        for (int g = 0; g < G; ++g) {
+        for (int g = 0; g < GL; ++g) {
           // 2^24 and 2^(e_ref - 127 - 5) undone in two steps: either alone could leave the range
-          const float f1 = __uint_as_float(static_cast<uint32_t>(e_ref[g]) << 23), f2 = a * (16777216.0f / (1 << kPShift));
+          const float f1 = __uint_as_float(e_ref[g] << 23), f2 = a * (16777216.0f / (1 << kPShift));
           float4 v[2];
           float* f = reinterpret_cast<float*>(v);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            f[2 * k] = fmaf(o[nt][g][k][c] * f2, f1, a * zsum[nt][g][c]);
-            f[2 * k + 1] = fmaf(o[nt][g][k][2 + c] * (f2 * 0.0625f), f1, a * zsum[nt][g][c]);
+            // (PAIR: the columns of the other group are of no use)
+            const float x = PAIR && own == 1 ? o[nt][G - 1][k][c] : o[nt][g][k][c], y = PAIR && own == 1 ? o[nt][G - 1][k][2 + c] : o[nt][g][k][2 + c];
+            f[2 * k] = fmaf(x * f2, f1, a * zsum[nt][g][c]);
+            f[2 * k + 1] = fmaf(y * (f2 * 0.0625f), f1, a * zsum[nt][g][c]);
           }
           // (a warp that saw nothing of a row has nothing to add, not zero times what it holds)
           if (m[nt][c] == -INFINITY && l[nt][c] == 0.0f) v[0] = v[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          float4* dst = reinterpret_cast<float4*>(&sm.o[warp][r][g * 64 + g8 * 8]);
+          float4* dst = reinterpret_cast<float4*>(&sm.o[warp][r][(PAIR ? own : g) * 64 + g8 * 8]);
           dst[0] = v[0];
           dst[1] = v[1];
         }
       }
-    __syncthreads();
+    ptx::named_bar_sync(1, kWorkers);
     if (!ok) break;
     // thread: eight columns of a row
     const bool alone = part.i1 - part.i0 == part.n;
-    for (int x = threadIdx.x; x < kRowsU * (D / 8); x += kThreads) {
+    for (int x = threadIdx.x; x < kRows * (D / 8); x += kWorkers) {
       const int r = x / (D / 8), col = (x % (D / 8)) * 8, rr = row0 + r;
       if (rr >= p.R) continue;
       float mt = -INFINITY, lt = 0.0f, v[8] = {};
@@ -599,9 +629,9 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
         const float2 ml = sm.ml[w][r];
         const float wgt = ml.x == -INFINITY ? (ml.y == 0.0f ? 0.0f : 1.0f) : ptx::ex2_approx(ml.x - mt);
         lt += wgt * ml.y;
-        const float4 a = *reinterpret_cast<const float4*>(&sm.o[w][r][col]), c = *reinterpret_cast<const float4*>(&sm.o[w][r][col + 4]);
-        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-        v[4] += c.x; v[5] += c.y; v[6] += c.z; v[7] += c.w;
+        const float4 y0 = *reinterpret_cast<const float4*>(&sm.o[w][r][col]), y1 = *reinterpret_cast<const float4*>(&sm.o[w][r][col + 4]);
+        v[0] += y0.x; v[1] += y0.y; v[2] += y0.z; v[3] += y0.w;
+        v[4] += y1.x; v[5] += y1.y; v[6] += y1.z; v[7] += y1.w;
       }
       if (alone) {
         const float inv = lt == 0.0f ? 0.0f : 1.0f / lt;
@@ -611,24 +641,19 @@ __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3) kv4_decode_kernel(c
                                           attn::pack16<FMT>(v[4] * inv, v[5] * inv), attn::pack16<FMT>(v[6] * inv, v[7] * inv)));
         if (W && col == 0) *reinterpret_cast<float2*>(p.row_ml + ((static_cast<int64_t>(b) * p.Hk + hk) * p.R + rr) * 2) = make_float2(mt, lt);
       } else {
-        const int64_t piece = (static_cast<int64_t>(blockIdx.x) + b * per_seq + part.unit) * kRowsU + r;
+        const int64_t piece = (static_cast<int64_t>(blockIdx.x) + b * per_seq + part.unit) * kRows + r;
         float4* dst = reinterpret_cast<float4*>(p.part_o + piece * D + col);
         dst[0] = make_float4(v[0], v[1], v[2], v[3]);
         dst[1] = make_float4(v[4], v[5], v[6], v[7]);
         if (col == 0) *reinterpret_cast<float2*>(p.part_ml + piece * 2) = make_float2(mt, lt);
       }
     }
-    __syncthreads();                                   // the next part's pieces overwrite these
+    ptx::named_bar_sync(1, kWorkers);                  // the next part's pieces overwrite these
   }
-  if (!ok) {
-    // the run was given up: this warp's copies land before the block's memory is handed on; noted once for the launch
-    volatile uint32_t never = 0;
-    for (int i = taken; i < requested; ++i)
-      ptx::mbar_wait(&sm.full[warp][i % Sm::kStages], static_cast<uint32_t>(i / Sm::kStages) & 1u, 100000000ull, &never);
-    if (threadIdx.x == 0 && atomicCAS(p.status, 0u, static_cast<uint32_t>(STATUS_TIMEOUT_PIPELINE)) == 0u) {
-      p.status[1] = 0u; p.status[2] = 400u; p.status[3] = 0u; p.status[4] = 0u; p.status[5] = 0u; p.status[6] = blockIdx.x;
-      __threadfence_system();
-    }
+  // a wait that ran out of time, noted once for the launch
+  if (!ok && threadIdx.x == 0 && atomicCAS(p.status, 0u, static_cast<uint32_t>(STATUS_TIMEOUT_PIPELINE)) == 0u) {
+    p.status[1] = 0u; p.status[2] = 400u; p.status[3] = 0u; p.status[4] = 0u; p.status[5] = 0u; p.status[6] = blockIdx.x;
+    __threadfence_system();
   }
 }
 
@@ -642,7 +667,7 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const DecodeParams p, 
   const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int hk = in_seq / p.chunks, rr = (in_seq - hk * p.chunks) * rows_unit + r;
   if (r >= rows_unit || rr >= p.R) return;
-  const int n = p.prefix[b + 1] - p.prefix[b], total = p.prefix[p.B] * per_seq, per = (total + ctas - 1) / ctas;
+  const int n = p.prefix[b + 1] - p.prefix[b], total = p.prefix[p.B] * per_seq, per = blocks_per_run(total, ctas);
   const int first = p.prefix[b] * per_seq + in_seq * n;
   const int tok = rr / p.group;
   uint16_t* dst = static_cast<uint16_t*>(p.out) + ((static_cast<int64_t>(b) * p.q_len + tok) * p.Hq + hk * p.group + (rr - tok * p.group)) * D + lane * kPer;
@@ -717,7 +742,7 @@ using namespace catcoc::kv4;
 
 namespace {
 struct DecodePlan {
-  int R, nt, chunks;
+  int R, rows, chunks;      // rows: of a unit, as the kernel is built for them
   int64_t units, blocks;     // blocks: an upper bound, by the block table
   int ctas;
   int64_t o_floats, ml_floats, prefix_ints, row_floats, score_floats;
@@ -732,8 +757,8 @@ bool decode_plan(const CatcocKv4Call& c, bool weights, DecodePlan& d) {
       c.max_pages <= 0 || c.window < 0 || c.sinks < 0 || static_cast<int64_t>(c.Hq / c.Hk) * c.q_len > 4096)
     return false;
   d.R = c.Hq / c.Hk * c.q_len;
-  d.nt = d.R <= 8 ? 1 : 2;
-  d.chunks = (d.R + 8 * d.nt - 1) / (8 * d.nt);
+  d.rows = d.R <= 4 && c.D == 128 ? 4 : d.R <= 8 ? 8 : 16;
+  d.chunks = (d.R + d.rows - 1) / d.rows;
   d.units = static_cast<int64_t>(c.B) * c.Hk * d.chunks;
   int64_t seq = c.max_pages;
   if (c.window > 0) seq = std::min<int64_t>(seq, (static_cast<int64_t>(c.window) + c.q_len + 62) / 64 + 1 + (static_cast<int64_t>(c.sinks) + 63) / 64);
@@ -741,10 +766,10 @@ bool decode_plan(const CatcocKv4Call& c, bool weights, DecodePlan& d) {
   if (d.blocks > (1ll << 30) || static_cast<int64_t>(c.max_pages) * kPage > (1ll << 24)) return false;
   int device = 0;
   cudaGetDevice(&device);
-  d.ctas = static_cast<int>(std::min<int64_t>(d.blocks, static_cast<int64_t>(catcoc_num_sms(device)) * (d.nt == 1 ? 4 : 3)));
-  const int64_t pieces = d.ctas + d.units, rows = 8 * d.nt;
-  d.o_floats = pieces * rows * c.D;
-  d.ml_floats = pieces * rows * 2;
+  d.ctas = static_cast<int>(std::min<int64_t>(d.blocks, static_cast<int64_t>(catcoc_num_sms(device)) * (d.rows == 16 ? 2 : 3)));
+  const int64_t pieces = d.ctas + d.units;
+  d.o_floats = pieces * d.rows * c.D;
+  d.ml_floats = pieces * d.rows * 2;
   d.prefix_ints = c.B + 1;
   d.row_floats = weights ? static_cast<int64_t>(c.B) * c.Hk * d.R * 2 : 0;
   d.score_floats = weights ? static_cast<int64_t>(c.B) * c.Hk * d.R * c.max_pages * kPage : 0;
@@ -788,11 +813,11 @@ extern "C" int catcoc_kv4_decode(const CatcocKv4Call* c, const void* q, const vo
   p.timeout_ns = timeout_ns ? timeout_ns : 10000000000ull;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   auto launch = [&](auto main_kernel, auto combine_kernel, size_t smem) -> int {
-    smem += static_cast<size_t>(B) * 8 + 128;
+    smem += 128;
     CATCOC_CUDA_OK(cudaFuncSetAttribute(main_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     CATCOC_CUDA_OK(launch_overlapped(main_kernel, dim3(static_cast<unsigned>(d.ctas)), dim3(kThreads), smem, stream, p));
-    CATCOC_CUDA_OK(launch_overlapped(combine_kernel, dim3(static_cast<unsigned>(d.units), static_cast<unsigned>((std::min(d.R, 8 * d.nt) + 3) / 4)), dim3(128), 0,
-                                     stream, p, 8 * d.nt, d.ctas));
+    CATCOC_CUDA_OK(launch_overlapped(combine_kernel, dim3(static_cast<unsigned>(d.units), static_cast<unsigned>((std::min(d.R, d.rows) + 3) / 4)), dim3(128), 0,
+                                     stream, p, d.rows, d.ctas));
     if (weights)
       CATCOC_CUDA_OK(launch_overlapped(kv4_weights_kernel, dim3(static_cast<unsigned>(B * Hk), static_cast<unsigned>((p.S + 255) / 256)), dim3(256),
                                        d.R * sizeof(float2), stream, p, weights, static_cast<int64_t>(c->S)));
@@ -800,11 +825,16 @@ extern "C" int catcoc_kv4_decode(const CatcocKv4Call* c, const void* q, const vo
   };
   auto by_rows = [&](auto dim, auto type) -> int {
     constexpr int kD = decltype(dim)::value, kF = decltype(type)::value;
-    if (d.nt == 1)
-      return weights ? launch(kv4_decode_kernel<kD, kF, 1, true>, kv4_combine_kernel<kD, kF, true>, sizeof(Smem<kD, 1>))
-                     : launch(kv4_decode_kernel<kD, kF, 1, false>, kv4_combine_kernel<kD, kF, false>, sizeof(Smem<kD, 1>));
-    return weights ? launch(kv4_decode_kernel<kD, kF, 2, true>, kv4_combine_kernel<kD, kF, true>, sizeof(Smem<kD, 2>))
-                   : launch(kv4_decode_kernel<kD, kF, 2, false>, kv4_combine_kernel<kD, kF, false>, sizeof(Smem<kD, 2>));
+    auto with = [&](auto eights, auto pair) -> int {
+      constexpr int kE = decltype(eights)::value;
+      constexpr bool kP = decltype(pair)::value;
+      return weights ? launch(kv4_decode_kernel<kD, kF, kE, kP, true>, kv4_combine_kernel<kD, kF, true>, sizeof(Smem<kD, kE, kP>))
+                     : launch(kv4_decode_kernel<kD, kF, kE, kP, false>, kv4_combine_kernel<kD, kF, false>, sizeof(Smem<kD, kE, kP>));
+    };
+    if constexpr (kD == 128) {
+      if (d.rows == 4) return with(std::integral_constant<int, 1>{}, std::true_type{});
+    }
+    return d.rows == 8 ? with(std::integral_constant<int, 1>{}, std::false_type{}) : with(std::integral_constant<int, 2>{}, std::false_type{});
   };
   const bool bf = fmt == CATCOC_FMT_BF16;
   if (D == 128) return bf ? by_rows(std::integral_constant<int, 128>{}, std::integral_constant<int, FMT_BF16>{}) : by_rows(std::integral_constant<int, 128>{}, std::integral_constant<int, FMT_F16>{});
