@@ -12,7 +12,9 @@
 // so that a code costs a mask (five instructions for eight codes of K, six for V's): four bits at the bottom of a half are the subnormal
 // code * 2^-24, those above them code * 2^-20, both exact operands. The 16 between them goes into q and into the result. q is brought into
 // the range of a half by a power of two per row, p s by one per group that follows the largest scale, so that the only rounding in
-// front of the accumulators is that of p s to 11 bits.
+// front of the accumulators is that of p s to 11 bits. For that rounding V's codes count from 8, o_c = sum_j (p_j s_jg) (code_jc - 8) +
+// sum_j p_j (z_jg + 8 s_jg), with 8 times the sum of the rounded p s taken off at the end (one product with ones a tile): counted from 0 it would
+// come multiplied by codes twice as large as the values, 6.2e-4 of an fp16 output where 2.4e-4 remain.
 //
 // S^T = K q^T has the tokens as rows of mma.m16n8k16; its accumulator, scaled, rounded and transposed by movmatrix, is the second operand of
 // O^T += V^T (p s). With up to four rows over two groups of channels (PAIR) the eight columns are four rows of each group, so that no lane
@@ -82,10 +84,17 @@ CATCOC_DEVICE Span span_of(int len, int q_len, int window, int sinks) {
   return s;
 }
 
-// Blocks of a CTA's run; stages take two, so runs of more than two are even
-CATCOC_DEVICE int blocks_per_run(int total, int ctas) {
-  const int per = (total + ctas - 1) / ctas;
-  return per > kSub ? (per + 1) & ~1 : per;
+// The list in runs, one a CTA: pairs of blocks, as many each and one more in the first ones (whose SMs are different ones), or single blocks
+// while there are no more of them than CTAs. Run c begins at run_begin(c); block x is in run run_of(x).
+CATCOC_DEVICE int run_begin(int c, int total, int ctas) {
+  if (total <= ctas) return min(c, total);
+  const int pairs = (total + kSub - 1) / kSub, each = pairs / ctas;
+  return min(total, kSub * (c * each + min(c, pairs - each * ctas)));
+}
+CATCOC_DEVICE int run_of(int x, int total, int ctas) {
+  if (total <= ctas) return x;
+  const int pairs = (total + kSub - 1) / kSub, each = pairs / ctas, more = pairs - each * ctas, y = x / kSub;
+  return y < more * (each + 1) ? y / (each + 1) : more + (y - more * (each + 1)) / each;   // (each is 0 only where all pairs are in the first runs)
 }
 
 CATCOC_DEVICE void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -161,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
     int sum = 0;
     for (int b = lane; b < p.B; b += 32) sum += span_at(seq_len(p.lens, b, p.max_pages * kPage, p.status)).count();
     const int total = __reduce_add_sync(0xffffffffu, sum) * per_seq;
-    const int begin = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * blocks_per_run(total, static_cast<int>(gridDim.x)), static_cast<int64_t>(total)));
+    const int begin = run_begin(blockIdx.x, total, static_cast<int>(gridDim.x));
     int behind = 0, start = 0, base = 0;
     for (int chunk = 0; chunk < p.B; chunk += 32) {
       const int b = chunk + lane, mine = b < p.B ? span_at(seq_len(p.lens, b, p.max_pages * kPage, p.status)).count() : 0;
@@ -190,8 +199,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
   }
   __syncthreads();
   const int total = sm.total;
-  const int per = blocks_per_run(total, static_cast<int>(gridDim.x));
-  const int begin = static_cast<int>(min(static_cast<int64_t>(blockIdx.x) * per, static_cast<int64_t>(total))), end = min(total, begin + per);
+  const int begin = run_begin(blockIdx.x, total, static_cast<int>(gridDim.x)), end = run_begin(blockIdx.x + 1, total, static_cast<int>(gridDim.x));
   // the part of the run that begins at list position `at`, in the sequence of `s` or behind it
   auto part_at = [&](int at, Part s) {
     while (s.base + s.n * per_seq <= at) {
@@ -315,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
       }
     }
     // m: largest raw score, as far as it is followed; m_neg: minus its score; limit: raw score from which on it moves
-    float o[NT][G][4][4] = {}, m[NT][2], m_neg[NT][2], limit[NT][2], l[NT][2] = {}, zsum[NT][GL][2] = {};
+    float o[NT][G][4][4] = {}, wsum[NT][GL][4] = {}, m[NT][2], m_neg[NT][2], limit[NT][2], l[NT][2] = {}, zsum[NT][GL][2] = {};
     uint32_t e_ref[GL];                               // exponent field that the scales of V are held against
     float vscale[GL];                                 // 2^(kPShift + 127 - e_ref)
 #pragma unroll
@@ -479,7 +487,10 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
             limit[nt][c] = mn + attn::kLazyRescale / qscale[nt][c];
             l[nt][c] *= alpha;
 #pragma unroll
-            for (int g = 0; g < GL; ++g) zsum[nt][g][c] *= alpha;
+            for (int g = 0; g < GL; ++g) {
+              zsum[nt][g][c] *= alpha;
+              wsum[nt][g][c] *= alpha * beta[g];
+            }
 #pragma unroll
             for (int g = 0; g < G; ++g)
 #pragma unroll
@@ -506,12 +517,13 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               w[e] = pr[e] * ps[i][g][e >> 1];
-              float z = bf16_hi(vpar[i][e >> 1][g]);
+              float z = fmaf(8.0f, bf16_lo(vpar[i][e >> 1][g]), bf16_hi(vpar[i][e >> 1][g]));
               if (!ALL && s[i][nt][e] == -INFINITY) { w[e] = 0.0f; z = 0.0f; }
               zsum[nt][g][e & 1] = fmaf(pr[e], z, zsum[nt][g][e & 1]);
             }
             pb[nt][g][0] = transpose8(half2_of(w[0], w[1]));
             pb[nt][g][1] = transpose8(half2_of(w[2], w[3]));
+            mma_f16(wsum[nt][g], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, pb[nt][g][0], pb[nt][g][1]);
           }
         }
         // O^T: rows g8 and g8 + 8 are the channels 64 g + 8 g8 + 2 k and + 1, tokens of the rows 2 t4, 2 t4 + 1, + 8, + 9
@@ -546,7 +558,8 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
         const int key0 = span.block(i + sub) * kPage + token0;
         const uint8_t* block = sm.stage[stage][sub];
         if (key0 + kItem - 1 <= pos_lo && (p.window == 0 || pos_hi - key0 < p.window || key0 + kItem <= p.sinks)) {
-          if constexpr (NT == 1) {
+          // (two tiles at once where their state fits the registers)
+          if constexpr (PAIR || (NT == 1 && G == 1)) {
             tiles(std::true_type{}, std::integral_constant<int, kItem / kTile>{}, block, token0, key0);
           } else {
 #pragma unroll 1
@@ -598,14 +611,15 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
         for (int g = 0; g < GL; ++g) {
           // 2^24 and 2^(e_ref - 127 - 5) undone in two steps: either alone could leave the range
           const float f1 = __uint_as_float(e_ref[g] << 23), f2 = a * (16777216.0f / (1 << kPShift));
+          const float eights = wsum[nt][g][c] * (a * (-8.0f / (1 << kPShift)));
           float4 v[2];
           float* f = reinterpret_cast<float*>(v);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             // (PAIR: the columns of the other group are of no use)
             const float x = PAIR && own == 1 ? o[nt][G - 1][k][c] : o[nt][g][k][c], y = PAIR && own == 1 ? o[nt][G - 1][k][2 + c] : o[nt][g][k][2 + c];
-            f[2 * k] = fmaf(x * f2, f1, a * zsum[nt][g][c]);
-            f[2 * k + 1] = fmaf(y * (f2 * 0.0625f), f1, a * zsum[nt][g][c]);
+            f[2 * k] = fmaf(fmaf(x, f2, eights), f1, a * zsum[nt][g][c]);
+            f[2 * k + 1] = fmaf(fmaf(y, f2 * 0.0625f, eights), f1, a * zsum[nt][g][c]);
           }
           // (a warp that saw nothing of a row has nothing to add, not zero times what it holds)
           if (m[nt][c] == -INFINITY && l[nt][c] == 0.0f) v[0] = v[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -667,13 +681,13 @@ __global__ void __launch_bounds__(128) kv4_combine_kernel(const DecodeParams p, 
   const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int hk = in_seq / p.chunks, rr = (in_seq - hk * p.chunks) * rows_unit + r;
   if (r >= rows_unit || rr >= p.R) return;
-  const int n = p.prefix[b + 1] - p.prefix[b], total = p.prefix[p.B] * per_seq, per = blocks_per_run(total, ctas);
+  const int n = p.prefix[b + 1] - p.prefix[b], total = p.prefix[p.B] * per_seq;
   const int first = p.prefix[b] * per_seq + in_seq * n;
   const int tok = rr / p.group;
   uint16_t* dst = static_cast<uint16_t*>(p.out) + ((static_cast<int64_t>(b) * p.q_len + tok) * p.Hq + hk * p.group + (rr - tok * p.group)) * D + lane * kPer;
   float m = -INFINITY, l = 0.0f, acc[kPer] = {};
   if (n > 0) {
-    const int c0 = first / per, c1 = (first + n - 1) / per;
+    const int c0 = run_of(first, total, ctas), c1 = run_of(first + n - 1, total, ctas);
     if (c0 == c1) return;                          // written by its CTA
     for (int base = c0; base <= c1; base += 32) {
       const int count = min(32, c1 + 1 - base);
@@ -753,7 +767,7 @@ struct DecodePlan {
 
 // false: a call that the kernel does not take
 bool decode_plan(const CatcocKv4Call& c, bool weights, DecodePlan& d) {
-  if (c.B <= 0 || c.B > 4096 || c.q_len <= 0 || c.q_len > 64 || c.Hk <= 0 || c.Hq <= 0 || c.Hq % c.Hk != 0 || (c.D != 64 && c.D != 128) || c.pages <= 0 ||
+  if (c.B <= 0 || c.B > 65536 || c.q_len <= 0 || c.q_len > 64 || c.Hk <= 0 || c.Hq <= 0 || c.Hq % c.Hk != 0 || (c.D != 64 && c.D != 128) || c.pages <= 0 ||
       c.max_pages <= 0 || c.window < 0 || c.sinks < 0 || static_cast<int64_t>(c.Hq / c.Hk) * c.q_len > 4096)
     return false;
   d.R = c.Hq / c.Hk * c.q_len;

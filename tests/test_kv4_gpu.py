@@ -6,7 +6,8 @@ Tolerances of the attention. The scores are sums of D products of whole codes in
 part: off by at most 2^-19 of M = scale log2(e) sum_c |q_c| (s code + |z|) (the matrix unit drops what lies 2^-23 under its largest term,
 16 terms and 8 steps, twice that for the fp32 steps around it), and exp2 is off by 2^-22: a probability is off by e = ln 2 (2^-19 M) + 2^-21 of
 itself, their sum by as much. The probabilities times scales are rounded to 11 bits (half a step: 2^-12), or where they lie 2^-23
-under the largest to 2^-38 of it, which n tokens can add up. The output is rounded once, by half a step of its type."""
+under the largest to 2^-38 of it, which n tokens can add up; they are the weights of code - 8. The fp32 sums of the codes and of the eights,
+which are as large as 16 p s, are off by 2^-20 of that. The output is rounded once, by half a step of its type."""
 import math
 
 import pytest
@@ -137,6 +138,7 @@ def _attend(q, cache, table, kv_lens, *, weights=None, q_len=1, window=None, sin
         for z in zeros:
             z[..., 1] = 0
         scaled = [kv4.dequantise_reference(c, z.flatten(-2).view(torch.uint8)).transpose(0, 1) for c, z in zip(codes, zeros)]   # s code [heads, n, D]
+        steps = [p.contiguous().view(torch.bfloat16).double().unflatten(-1, (-1, 2))[..., 0].repeat_interleave(64, -1).transpose(0, 1) for p in params]
         offs = [p.contiguous().view(torch.bfloat16).double().unflatten(-1, (-1, 2))[..., 1].abs().repeat_interleave(64, -1).transpose(0, 1) for p in params]
         k_all, v_all = kv4.kv4_read_reference(cache, table[b:b + 1], kv_lens[b:b + 1])
         k_all, v_all = k_all[0, :, :n], v_all[0, :, :n]
@@ -153,10 +155,11 @@ def _attend(q, cache, table, kv_lens, *, weights=None, q_len=1, window=None, sin
             big = (torch.einsum("hgd,hnd->hgn", x.abs(), scaled[0][:, seen] + offs[0][:, seen]) * sc * 1.4427).amax(-1)       # [heads, group]
             prob = torch.softmax(torch.einsum("hgd,hnd->hgn", x, k_all[:, seen]) * sc, -1)
             e = 2 * (math.log(2) * big * 2.0 ** -19 + 2.0 ** -21)                                                                 # [heads, group]
-            sc_v = torch.einsum("hgn,hnd->hgd", prob, scaled[1][:, seen])
-            abs_v = sc_v + torch.einsum("hgn,hnd->hgd", prob, offs[1][:, seen])
+            unit = steps[1][:, seen]                                                                                              # s
+            centred = torch.einsum("hgn,hnd->hgd", prob, (scaled[1][:, seen] - 8 * unit).abs())
+            abs_v = torch.einsum("hgn,hnd->hgd", prob, scaled[1][:, seen] + offs[1][:, seen]) + 16 * torch.einsum("hgn,hnd->hgd", prob, unit)
             floor = 2.0 ** -38 * 15 * int(seen.sum()) * scaled[1][:, seen].amax(1)[:, None]
-            tol = (2.0 ** -12 * sc_v + e[..., None] * abs_v + floor).view(heads * group, d) + eps / 2 * want[b * q_len + t].abs() + 1e-30
+            tol = (2.0 ** -12 * centred + (e[..., None] + 2.0 ** -20) * abs_v + floor).view(heads * group, d) + eps / 2 * want[b * q_len + t].abs() + 1e-30
             off = (out[b * q_len + t].double() - want[b * q_len + t]).abs()
             assert (off <= tol).all(), (b, t, float((off / tol).max()))
     if weights is not None:

@@ -196,7 +196,7 @@ def test_the_library_refuses_too():
     assert run(evict, 9, sinks=3) == N.E_BAD_ARG and run(evict, 9, S=127) == N.E_BAD_ARG and run(evict, 9, keep=0) == N.E_BAD_ARG
     assert run(evict, 9, keep=100, out_pages=1) == N.E_BAD_ARG and run(evict, 9, keep=100, S_out=99) == N.E_BAD_ARG
     assert run(evict, 9, D=32) == N.E_UNSUPPORTED and run(evict, 9, odd=0) == N.E_ALIGNMENT
-    for bad in (dict(Hq=3, Hk=2), dict(q_len=65), dict(q_len=0), dict(D=96), dict(B=4097), dict(q_len=64, Hq=128), dict(max_pages=1 << 19), dict(window=-1),
+    for bad in (dict(Hq=3, Hk=2), dict(q_len=65), dict(q_len=0), dict(D=96), dict(B=65537), dict(q_len=64, Hq=128), dict(max_pages=1 << 19), dict(window=-1),
                 dict(sinks=-1)):
         assert space(**bad) == -1 and run(decode, 8, **bad) == N.E_BAD_ARG
     assert run(decode, 8, scale=0.0) == N.E_UNSUPPORTED and run(decode, 8, scale=float("nan")) == N.E_UNSUPPORTED
