@@ -47,13 +47,14 @@ CATCOC_DEVICE int seq_len(const int* lens, int b, int capacity, uint32_t* status
   return n;
 }
 
-// Page `i` of a sequence, or -1
-CATCOC_DEVICE int page_of(const int* table, int64_t row, int i, int pages, uint32_t* status) {
-  const int page = table[row + i];
+// A block table's entry, -1 where it names no page
+CATCOC_DEVICE int checked_page(int page, int pages, uint32_t* status) {
   if (static_cast<uint32_t>(page) < static_cast<uint32_t>(pages)) return page;
   note(status, kErrPage, page, pages);
   return -1;
 }
+// Page `i` of a sequence, or -1
+CATCOC_DEVICE int page_of(const int* table, int64_t row, int i, int pages, uint32_t* status) { return checked_page(table[row + i], pages, status); }
 
 CATCOC_DEVICE float bf16_lo(uint32_t pair) { return __uint_as_float(pair << 16); }
 CATCOC_DEVICE float bf16_hi(uint32_t pair) { return __uint_as_float(pair & 0xffff0000u); }

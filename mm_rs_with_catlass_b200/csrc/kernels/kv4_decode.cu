@@ -5,7 +5,7 @@
 // pieces of a unit that lies in several runs are merged by a second kernel, and a third one adds the probabilities to the caller's sums.
 //
 //   warps 0..3  32 tokens of a stage (two blocks) each, with a softmax and an O of their own; merged at the end of a unit
-//   warp 4      producer: one bulk copy a block (72 D bytes) into a ring of stages
+//   warp 4      producer: walks the run; what the next part is and its rows of q, and one bulk copy a block (72 D bytes) into a ring of stages
 //
 // Both products run on codes, without their values: with scales and zeros constant over a group g of channels,
 //   q . k_j = sum_g s_jg (sum_c q_c code_jc) + z_jg (sum_c q_c),   o_c = sum_j (p_j s_jg) code_jc + sum_j p_j z_jg,
@@ -112,6 +112,13 @@ CATCOC_DEVICE uint32_t half2_of(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+CATCOC_DEVICE bool vote_any(bool pred) {           // of the consumer warps
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+               : "=r"(r) : "r"(static_cast<uint32_t>(pred)), "n"(kWorkers) : "memory");
+  return r != 0u;
+}
+
 // Row of a matrix instruction -> token of the tile. Two tokens of a pair are swapped in every other pair, so that the rows that four
 // lanes read of V lie in both halves of the banks (K's stay free of conflicts).
 CATCOC_DEVICE int token_of(int row) { return row ^ ((row >> 1) & 1); }
@@ -133,14 +140,16 @@ struct Geo {
 template <int D, int NT, bool PAIR>
 struct Smem {
   using Ge = Geo<D, NT, PAIR>;
-  alignas(128) uint8_t stage[Ge::kStages][kSub][Block<D>::kBytes];
+  alignas(16) uint8_t stage[Ge::kStages][kSub][Block<D>::kBytes];
   float o[kWarps][Ge::kRows][D + 4];   // (4: the lanes of a warp store to different banks)
   float2 ml[kWarps][Ge::kRows];
-  uint64_t full[Ge::kStages], empty[Ge::kStages];
+  alignas(16) uint16_t q[2][Ge::kRows * D];   // the rows of a part, and of the one behind it
+  Part part[2];                        // n = 0: the run is at its end
+  uint64_t full[Ge::kStages], empty[Ge::kStages], part_full[2], part_empty[2];
   uint32_t abort_flag, failed[kWarps];
-  int total;                           // blocks of the list
-  Part start;                          // the sequence in which the run begins
 };
+static_assert(3 * (sizeof(Smem<128, 1, false>) + 1024) <= 228 * 1024 && 3 * (sizeof(Smem<64, 1, false>) + 1024) <= 228 * 1024 &&
+              2 * (sizeof(Smem<128, 2, false>) + 1024) <= 228 * 1024, "the CTAs of an SM share its memory");
 
 // D: head dimension, FMT: type of q and out, W: the scores are written for the weights
 template <int D, int FMT, int NT, bool PAIR, bool W>
@@ -151,8 +160,8 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
   static_assert(!PAIR || (NT == 1 && L::kGroups == 2));
   constexpr int G = Ge::G, kRows = Ge::kRows;
   constexpr int GL = PAIR ? 1 : G;               // groups of channels that a lane's columns stand for
-  extern __shared__ uint8_t smem_raw[];
-  Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~static_cast<uintptr_t>(127));
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   volatile uint32_t* abort_flag = &sm.abort_flag;
   const int per_seq = p.Hk * p.chunks;            // units of a sequence
@@ -160,20 +169,26 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < Ge::kStages; ++s) { ptx::mbar_init(&sm.full[s], 1); ptx::mbar_init(&sm.empty[s], kWarps); }
+    for (int s = 0; s < 2; ++s) { ptx::mbar_init(&sm.part_full[s], 1); ptx::mbar_init(&sm.part_empty[s], kWarps); }
     sm.abort_flag = 0;
     ptx::mbar_fence_init();
   }
+  __syncthreads();
   ptx::grid_dependency_wait();
   ptx::launch_dependents();
+  uint32_t step = 0, parts = 0;                   // stages and parts so far
+
   if (warp == kWarps) {
+    // ------------------------------ producer ------------------------------
     // the blocks of all sequences, and the sequence in which this CTA's run begins
     int sum = 0;
     for (int b = lane; b < p.B; b += 32) sum += span_at(seq_len(p.lens, b, p.max_pages * kPage, p.status)).count();
     const int total = __reduce_add_sync(0xffffffffu, sum) * per_seq;
     const int begin = run_begin(blockIdx.x, total, static_cast<int>(gridDim.x));
-    int behind = 0, start = 0, base = 0;
+    int behind = 0;
+    Part part{0, 0, 0, 0, 0, 0, 0};
     for (int chunk = 0; chunk < p.B; chunk += 32) {
-      const int b = chunk + lane, mine = b < p.B ? span_at(seq_len(p.lens, b, p.max_pages * kPage, p.status)).count() : 0;
+      const int b = chunk + lane, len = b < p.B ? seq_len(p.lens, b, p.max_pages * kPage, p.status) : 0, mine = span_at(len).count();
       int n = mine;
 #pragma unroll
       for (int o = 1; o < 32; o *= 2) {
@@ -182,52 +197,67 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
       }
       n += behind;
       if (blockIdx.x == 0 && b < p.B) p.prefix[b + 1] = n;
-      const uint32_t hit = __ballot_sync(0xffffffffu, b < p.B && (n - mine) * per_seq <= begin && begin < n * per_seq);
+      const uint32_t hit = __ballot_sync(0xffffffffu, (n - mine) * per_seq <= begin && begin < n * per_seq);
       if (hit != 0u) {
-        start = chunk + __ffs(hit) - 1;
-        base = __shfl_sync(0xffffffffu, (n - mine) * per_seq, __ffs(hit) - 1);
+        const int from = __ffs(hit) - 1;
+        part.b = chunk + from;
+        part.base = __shfl_sync(0xffffffffu, (n - mine) * per_seq, from);
+        part.n = __shfl_sync(0xffffffffu, mine, from);
+        part.len = __shfl_sync(0xffffffffu, len, from);
         if (blockIdx.x != 0) break;
       }
       behind = __shfl_sync(0xffffffffu, n, 31);
     }
-    if (lane == 0) {
-      if (blockIdx.x == 0) p.prefix[0] = 0;
-      const int len = seq_len(p.lens, start, p.max_pages * kPage, p.status);
-      sm.total = total;
-      sm.start = Part{start, base, span_at(len).count(), len, 0, 0, 0};
+    if (blockIdx.x == 0 && lane == 0) p.prefix[0] = 0;
+    const int end = run_begin(blockIdx.x + 1, total, static_cast<int>(gridDim.x));
+    // the part of the run that begins at list position `at`, in the sequence of `s` or behind it
+    auto settle = [&](Part& s, int at) {
+      while (s.base + s.n * per_seq <= at) {
+        s.base += s.n * per_seq;
+        ++s.b;
+        s.len = seq_len(p.lens, s.b, p.max_pages * kPage, p.status);
+        s.n = span_at(s.len).count();
+      }
+      s.unit = (at - s.base) / s.n;
+      s.i0 = at - s.base - s.unit * s.n;
+      s.i1 = min(s.n, s.i0 + end - at);
+    };
+    // names of 32 blocks from block i on, as the table has them
+    auto names = [&](const Part& s, int i) { return i + lane < s.i1 ? p.table[static_cast<int64_t>(s.b) * p.max_pages + span_at(s.len).block(i + lane)] : 0; };
+    int raw = 0;
+    if (begin < end) {
+      settle(part, begin);
+      raw = names(part, part.i0);
     }
-  }
-  __syncthreads();
-  const int total = sm.total;
-  const int begin = run_begin(blockIdx.x, total, static_cast<int>(gridDim.x)), end = run_begin(blockIdx.x + 1, total, static_cast<int>(gridDim.x));
-  // the part of the run that begins at list position `at`, in the sequence of `s` or behind it
-  auto part_at = [&](int at, Part s) {
-    while (s.base + s.n * per_seq <= at) {
-      s.base += s.n * per_seq;
-      ++s.b;
-      s.len = seq_len(p.lens, s.b, p.max_pages * kPage, p.status);
-      s.n = span_at(s.len).count();
-    }
-    s.unit = (at - s.base) / s.n;
-    s.i0 = at - s.base - s.unit * s.n;
-    s.i1 = min(s.n, s.i0 + end - at);
-    return s;
-  };
-  uint32_t step = 0;                              // stages so far
-  Part part = sm.start;
-
-  if (warp == kWarps) {
-    // ------------------------------ producer ------------------------------
     bool ok = true;
-    for (int at = begin; ok && at < end; at += part.i1 - part.i0) {
-      part = part_at(at, part);
-      const Span span = span_at(part.len);
-      const int hk = part.unit / p.chunks;
-      int ids = -1;
+    for (int at = begin; ok && at < end; ++parts) {
+      const int hk = part.unit / p.chunks, row0 = (part.unit - hk * p.chunks) * kRows, rows = min(kRows, p.R - row0);
+      // what the part is, and its rows of q: those of a new token are consecutive heads
+      const uint32_t place = parts & 1u;
+      ok = ptx::mbar_wait(&sm.part_empty[place], ((parts >> 1) & 1u) ^ 1u, p.timeout_ns, abort_flag);
+      if (!ok) break;
+      if (lane == 0) {
+        sm.part[place] = part;
+        ptx::mbar_expect_tx(&sm.part_full[place], static_cast<uint32_t>(rows * D * 2));
+        for (int r = row0; r < row0 + rows;) {
+          const int tok = r / p.group, next = min(row0 + rows, (tok + 1) * p.group);
+          ptx::bulk_load_1d(sm.q[place] + (r - row0) * D,
+                            static_cast<const uint16_t*>(p.q) + ((static_cast<int64_t>(part.b) * p.q_len + tok) * p.Hq + hk * p.group + (r - tok * p.group)) * D,
+                            static_cast<uint32_t>((next - r) * D * 2), &sm.part_full[place]);
+          r = next;
+        }
+      }
+      __syncwarp();
+      at += part.i1 - part.i0;
+      Part next = part;
+      int ids = -1, next_raw = 0;
       for (int i = part.i0; i < part.i1; i += kSub, ++step) {
         // the names of 32 blocks at a time, so that no copy waits for its own
         const int k = (i - part.i0) & 31;
-        if (k == 0) ids = i + lane < part.i1 ? page_of(p.table, static_cast<int64_t>(part.b) * p.max_pages, span.block(i + lane), p.pages, p.status) : -1;
+        if (k == 0) {
+          if (i > part.i0) raw = names(part, i);
+          ids = i + lane < part.i1 ? checked_page(raw, p.pages, p.status) : -1;
+        }
         const uint32_t stage = step % Ge::kStages;
         ok = ptx::mbar_wait(&sm.empty[stage], ((step / Ge::kStages) & 1u) ^ 1u, p.timeout_ns, abort_flag);
         if (!ok) break;
@@ -247,7 +277,19 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
               ptx::bulk_load_1d(sm.stage[stage][s], p.cache + (static_cast<int64_t>(page[s]) * p.Hk + hk) * L::kBytes, L::kBytes, &sm.full[stage]);
         }
         __syncwarp();
+        // (behind the first copies: the next part and its names, under way while this one's are used)
+        if (i == part.i0 && at < end) {
+          settle(next, at);
+          next_raw = names(next, next.i0);
+        }
       }
+      part = next;
+      raw = next_raw;
+    }
+    if (ok) ok = ptx::mbar_wait(&sm.part_empty[parts & 1u], ((parts >> 1) & 1u) ^ 1u, p.timeout_ns, abort_flag);
+    if (ok && lane == 0) {
+      sm.part[parts & 1u].n = 0;
+      ptx::mbar_arrive(&sm.part_full[parts & 1u]);
     }
     if (!ok || *abort_flag != 0) {
       // the run was given up: the copies that are still on their way land before the block's memory is handed on
@@ -255,6 +297,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
       volatile uint32_t never = 0;
       for (uint32_t i = step > Ge::kStages ? step - Ge::kStages : 0; i < step; ++i)
         ptx::mbar_wait(&sm.full[i % Ge::kStages], (i / Ge::kStages) & 1u, 100000000ull, &never);
+      for (uint32_t i = parts > 2u ? parts - 2u : 0u; i < parts; ++i) ptx::mbar_wait(&sm.part_full[i & 1u], (i >> 1) & 1u, 100000000ull, &never);
     }
     return;
   }
@@ -265,8 +308,16 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
   const int sub = warp / (kWarps / kSub), token0 = (warp % (kWarps / kSub)) * kItem;   // this warp's block of a stage, and its tokens there
   auto row_of = [&](int nt, int c) { return PAIR ? 2 * (t4 & 1) + c : nt * 8 + 2 * t4 + c; };   // row of the unit that a lane's column stands for
   bool ok = true;
-  for (int at = begin; at < end && ok; at += part.i1 - part.i0) {
-    part = part_at(at, part);
+  for (;; ++parts) {
+    // (every warp takes all barriers of all parts, also after a failed wait; all leave together. The vote is also the barrier behind which
+    // the merge's memory is written again.)
+    const uint32_t place = parts & 1u;
+    ok = ptx::mbar_wait(&sm.part_full[place], (parts >> 1) & 1u, p.timeout_ns, abort_flag);
+    if (!ok && lane == 0) *abort_flag = 1;
+    ok = !vote_any(!ok);
+    if (!ok) break;
+    const Part part = sm.part[place];
+    if (part.n == 0) break;
     const int b = part.b, len = part.len;
     const Span span = span_at(len);
     const int hk = part.unit / p.chunks, row0 = (part.unit - hk * p.chunks) * kRows;   // first row of the unit among the R of its head
@@ -275,14 +326,13 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
     float qscale[NT][2], qsum[NT][GL][2];             // of the rows of this lane's columns: score = qscale * raw score
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = row0 + (PAIR ? g8 & 3 : nt * 8 + g8);
-      const int tok = r / p.group;
-      const uint16_t* src = static_cast<const uint16_t*>(p.q) + ((static_cast<int64_t>(b) * p.q_len + tok) * p.Hq + hk * p.group + (r - tok * p.group)) * D;
+      const int row = PAIR ? g8 & 3 : nt * 8 + g8;
+      const uint16_t* src = sm.q[place] + row * D;
       float x[2 * G][8], mx = 0.0f, sum[G] = {};
 #pragma unroll
       for (int i = 0; i < 2 * G; ++i) {
         uint4 raw = make_uint4(0, 0, 0, 0);
-        if (r < p.R) raw = *reinterpret_cast<const uint4*>(src + (i % G) * 64 + (2 * t4 + i / G) * 8);
+        if (row0 + row < p.R) raw = *reinterpret_cast<const uint4*>(src + (i % G) * 64 + (2 * t4 + i / G) * 8);
         const uint32_t u[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -322,6 +372,8 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
         for (int g = 0; g < GL; ++g) qsum[nt][g][c] = __shfl_sync(0xffffffffu, sum[g], from);
       }
     }
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(&sm.part_empty[place]);
     // m: largest raw score, as far as it is followed; m_neg: minus its score; limit: raw score from which on it moves
     float o[NT][G][4][4] = {}, wsum[NT][GL][4] = {}, m[NT][2], m_neg[NT][2], limit[NT][2], l[NT][2] = {}, zsum[NT][GL][2] = {};
     uint32_t e_ref[GL];                               // exponent field that the scales of V are held against
@@ -595,7 +647,6 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
       }
     if (!ok && lane == 0) *abort_flag = 1;
     if (lane == 0) sm.failed[warp] = ok ? 0u : 1u;
-    // (every warp walks the same parts and takes all barriers, also after a failed wait; all leave together)
     ptx::named_bar_sync(1, kWorkers);
     ok = (sm.failed[0] | sm.failed[1] | sm.failed[2] | sm.failed[3]) == 0u;
 #pragma unroll
@@ -662,7 +713,6 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
         if (col == 0) *reinterpret_cast<float2*>(p.part_ml + piece * 2) = make_float2(mt, lt);
       }
     }
-    ptx::named_bar_sync(1, kWorkers);                  // the next part's pieces overwrite these
   }
   // a wait that ran out of time, noted once for the launch
   if (!ok && threadIdx.x == 0 && atomicCAS(p.status, 0u, static_cast<uint32_t>(STATUS_TIMEOUT_PIPELINE)) == 0u) {
@@ -827,7 +877,6 @@ extern "C" int catcoc_kv4_decode(const CatcocKv4Call* c, const void* q, const vo
   p.timeout_ns = timeout_ns ? timeout_ns : 10000000000ull;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
   auto launch = [&](auto main_kernel, auto combine_kernel, size_t smem) -> int {
-    smem += 128;
     CATCOC_CUDA_OK(cudaFuncSetAttribute(main_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     CATCOC_CUDA_OK(launch_overlapped(main_kernel, dim3(static_cast<unsigned>(d.ctas)), dim3(kThreads), smem, stream, p));
     CATCOC_CUDA_OK(launch_overlapped(combine_kernel, dim3(static_cast<unsigned>(d.units), static_cast<unsigned>((std::min(d.R, d.rows) + 3) / 4)), dim3(128), 0,
