@@ -76,7 +76,8 @@ struct WindowParams {
 
 struct Bars {
   uint64_t q_full[kTiles], q_empty[kTiles], kv_full[kMaxSlots], kv_empty[kMaxSlots], s_full[kTiles], s_free[kTiles], p_half[kTiles], p_full[kTiles], pv_done[kTiles];
-  uint32_t tmem_base, abort_flag;
+  uint64_t drain[2];                               // of an issuer whose launch was given up: its products have retired
+  uint32_t tmem_base, abort_flag, kv_sent, q_sent[kTiles];
 };
 
 CATCOC_DEVICE void fail(const WindowParams& p, uint32_t what, uint32_t a) {
@@ -170,6 +171,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) { ptx::mbar_init(&bars->kv_full[s], 1); ptx::mbar_init(&bars->kv_empty[s], kIssuers); }
     for (int t = 0; t < kTiles; ++t) {
+      ptx::mbar_init(&bars->drain[t], 1);
+      bars->q_sent[t] = 0;
       ptx::mbar_init(&bars->q_full[t], 1);
       ptx::mbar_init(&bars->q_empty[t], 1);
       ptx::mbar_init(&bars->s_full[t], 1);
@@ -179,6 +182,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       ptx::mbar_init(&bars->p_full[t], 4);         // ... of all of them
     }
     bars->abort_flag = 0;
+    bars->kv_sent = 0;
     ptx::mbar_fence_init();
     ptx::prefetch_tmap(&p.tm_q); ptx::prefetch_tmap(&p.tm_k); ptx::prefetch_tmap(&p.tm_v);
   }
@@ -201,6 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
       for (int t = 0; ok && t < kTiles; ++t) {
         ok = ptx::mbar_wait(&bars->q_empty[t], (count & 1u) ^ 1u, p.timeout_ns, abort_flag);
         if (ok && ptx::elect_one()) {
+          bars->q_sent[t] = count + 1u;
           ptx::mbar_expect_tx(&bars->q_full[t], kQBytes);
           for (int d = 0; d < kDB; ++d) ptx::tma_load_3d(sq + t * kQBytes + d * kBlockBytes, &p.tm_q, &bars->q_full[t], d * 64, w.q0 + t * kBQ, w.bh);
         }
@@ -210,6 +215,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
         const uint32_t item = base + static_cast<uint32_t>(i), slot = item % kSlots;
         ok = ptx::mbar_wait(&bars->kv_empty[slot], ((item / kSlots) & 1u) ^ 1u, p.timeout_ns, abort_flag);
         if (ok && ptx::elect_one()) {
+          bars->kv_sent = item + 1u;
           ptx::mbar_expect_tx(&bars->kv_full[slot], kSlotBytes);
           const CUtensorMap* tm = (i & 1) ? &p.tm_v : &p.tm_k;
           for (int d = 0; d < kDB; ++d)
@@ -439,6 +445,21 @@ __global__ void __launch_bounds__(kThreads, 1) window_attn_kernel(const __grid_c
 
   ptx::tcgen05_fence_before();
   __syncthreads();
+  if (*abort_flag != 0) {
+    // the launch was given up: copies on their way land, and products retire, before the block's memory is handed on
+    volatile uint32_t never = 0;
+    if (warp == kProducerWarp) {
+      const uint32_t sent = bars->kv_sent;
+      for (uint32_t i = sent > kSlots ? sent - kSlots : 0u; i < sent; ++i) ptx::mbar_wait(&bars->kv_full[i % kSlots], (i / kSlots) & 1u, 100000000ull, &never);
+      for (int t = 0; t < kTiles; ++t)
+        if (bars->q_sent[t] != 0u) ptx::mbar_wait(&bars->q_full[t], (bars->q_sent[t] - 1u) & 1u, 100000000ull, &never);
+    } else if (warp >= kIssuerWarp && warp < kIssuerWarp + kIssuers) {
+      if (ptx::elect_one()) ptx::tcgen05_commit(&bars->drain[warp - kIssuerWarp]);
+      __syncwarp();
+      ptx::mbar_wait(&bars->drain[warp - kIssuerWarp], 0u, 100000000ull, &never);
+    }
+    __syncthreads();
+  }
   ptx::tcgen05_fence_after();
   if (warp == kIssuerWarp) ptx::tmem_dealloc(tmem, kTmemCols);
 }
