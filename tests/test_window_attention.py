@@ -73,6 +73,13 @@ def test_refusals():
     assert call(16, 16, 16, 16, None, 1, 1, 1, 400, 300, 64, N.FMT_BF16, 1, 0, 1.0, 16, 0, None) == N.E_BAD_ARG
 
 
+def test_few_rows_want_an_aligned_output():
+    """Few query rows: they are stored 16 bytes at a time."""
+    at = 1 << 20
+    call = N.lib().catcoc_window_attention
+    assert call(at, at, at, at + 8, at, 1, 4, 1, 1, 300, 64, N.FMT_BF16, 64, 4, 1.0, at, 0, None) == N.E_ALIGNMENT
+
+
 def test_scratch_goes_by_what_is_visible():
     assert _scratch(16, 32, 8, 1, 4096, 128, 64, 0) == (True, 0)                   # two blocks a sequence: whole runs
     assert _scratch(1, 8, 8, 512, 16384, 128, 4096, 64)[1] > 0                     # 34 blocks a tile, few tiles: slices
