@@ -401,10 +401,6 @@ CATCOC_DEVICE void bulk_load_1d(void* smem_dst, const void* gsrc, uint32_t bytes
       ::"r"(smem_u32(smem_dst)), "l"(gsrc), "r"(bytes), "r"(smem_u32(bar))
       : "memory");
 }
-// Asks for global memory to be brought into the L2 (16-byte aligned, size a multiple of 16)
-CATCOC_DEVICE void bulk_prefetch_l2(const void* gsrc, uint32_t bytes) {
-  asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(gsrc), "r"(bytes) : "memory");
-}
 // Descriptor of an unswizzled K-major block whose rows are 16 bytes: 8 rows form one contiguous
 // 128-byte core matrix, successive groups of 8 rows are `sbo_bytes` apart.
 CATCOC_DEVICE uint64_t make_smem_desc_noswizzle(uint32_t smem_addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {

@@ -367,7 +367,6 @@ def _serve(seed, steps=40, keep=96):
     """A short serving loop: a prompt, then steps that append, attend with a window's worth of sums, and evict when there is no room."""
     lens = [150, 70, 1]
     cache, table, kv_lens, k, v, ends, g = _make(lens, 2, 128, seed=seed, width=4)
-    tables = (table, torch.empty(0))
     return cache, table, kv_lens, k, v, ends, g, keep, steps
 
 
