@@ -4,7 +4,7 @@
 // once for all of them. The blocks of all units form one list, by the lengths on the device, that is cut into equal runs over the CTAs;
 // pieces of a unit that lies in several runs are merged by a second kernel, and a third one adds the probabilities to the caller's sums.
 //
-//   warps 0..3  32 tokens of a stage (two blocks) each, with a softmax and an O of their own; merged at the end of a unit
+//   warps 0..3  a quarter of a stage's tokens each (four blocks, or two), with a softmax and an O of their own; merged at the end of a unit
 //   warp 4      producer: walks the run; what the next part is and its rows of q, and one bulk copy a block (72 D bytes) into a ring of stages
 //
 // Both products run on codes, without their values: with scales and zeros constant over a group g of channels,
@@ -43,8 +43,8 @@ namespace kv4 {
 constexpr int kWarps = 4;                          // consumer warps
 constexpr int kThreads = 32 * (kWarps + 1), kWorkers = 32 * kWarps;
 constexpr int kTile = 16;                          // tokens of a matrix instruction
-constexpr int kSub = 2;                            // blocks of a stage
-constexpr int kItem = kSub * kPage / kWarps;       // tokens of a stage that a warp takes
+constexpr int kTilesBlock = kPage / kTile;
+constexpr int kPair = 2;                           // blocks that a run is a multiple of
 constexpr int kPShift = 5;                         // p s is held times 2^(5 - e), e: exponent of the largest scale; p <= 2^8, so below 2^14
 
 struct DecodeParams {
@@ -88,12 +88,12 @@ CATCOC_DEVICE Span span_of(int len, int q_len, int window, int sinks) {
 // while there are no more of them than CTAs. Run c begins at run_begin(c); block x is in run run_of(x).
 CATCOC_DEVICE int run_begin(int c, int total, int ctas) {
   if (total <= ctas) return min(c, total);
-  const int pairs = (total + kSub - 1) / kSub, each = pairs / ctas;
-  return min(total, kSub * (c * each + min(c, pairs - each * ctas)));
+  const int pairs = (total + kPair - 1) / kPair, each = pairs / ctas;
+  return min(total, kPair * (c * each + min(c, pairs - each * ctas)));
 }
 CATCOC_DEVICE int run_of(int x, int total, int ctas) {
   if (total <= ctas) return x;
-  const int pairs = (total + kSub - 1) / kSub, each = pairs / ctas, more = pairs - each * ctas, y = x / kSub;
+  const int pairs = (total + kPair - 1) / kPair, each = pairs / ctas, more = pairs - each * ctas, y = x / kPair;
   return y < more * (each + 1) ? y / (each + 1) : more + (y - more * (each + 1)) / each;   // (each is 0 only where all pairs are in the first runs)
 }
 
@@ -134,13 +134,18 @@ template <int D, int NT, bool PAIR>
 struct Geo {
   static constexpr int G = Block<D>::kGroups;
   static constexpr int kRows = PAIR ? 4 : 8 * NT;
-  static constexpr int kStages = D == 128 ? 3 : 5;
-  static constexpr int kCtas = NT == 1 ? 3 : 2;    // of an SM
+  // Tiles at once, blocks of a stage, CTAs of an SM: with few rows the chains of a tile (product, exp2, rounding, transpose, product) leave
+  // most issue slots empty, and four tiles at once in two CTAs of 168 registers pass two at once in three of 128: 16 x 8 heads x 4096 tokens,
+  // four rows, 27.2 -> 25.9 us (one at once in four of 96: 30.0), eight rows, two tiles, 29.2 -> 27.9, D = 64 20.0 -> 18.9.
+  static constexpr int kTiles = NT == 2 ? 1 : PAIR || G == 1 ? 4 : 2;
+  static constexpr int kSub = NT == 2 ? 2 : 4;     // blocks of a stage
+  static constexpr int kStages = NT == 2 ? 3 : 2;
+  static constexpr int kCtas = 2;                  // of an SM
 };
 template <int D, int NT, bool PAIR>
 struct Smem {
   using Ge = Geo<D, NT, PAIR>;
-  alignas(16) uint8_t stage[Ge::kStages][kSub][Block<D>::kBytes];
+  alignas(16) uint8_t stage[Ge::kStages][Ge::kSub][Block<D>::kBytes];
   float o[kWarps][Ge::kRows][D + 4];   // (4: the lanes of a warp store to different banks)
   float2 ml[kWarps][Ge::kRows];
   alignas(16) uint16_t q[2][Ge::kRows * D];   // the rows of a part, and of the one behind it
@@ -148,8 +153,7 @@ struct Smem {
   uint64_t full[Ge::kStages], empty[Ge::kStages], part_full[2], part_empty[2];
   uint32_t abort_flag, failed[kWarps];
 };
-static_assert(3 * (sizeof(Smem<128, 1, false>) + 1024) <= 228 * 1024 && 3 * (sizeof(Smem<64, 1, false>) + 1024) <= 228 * 1024 &&
-              2 * (sizeof(Smem<128, 2, false>) + 1024) <= 228 * 1024, "the CTAs of an SM share its memory");
+static_assert(2 * (sizeof(Smem<128, 2, false>) + 1024) <= 228 * 1024 && 2 * (sizeof(Smem<128, 1, false>) + 1024) <= 228 * 1024, "the CTAs of an SM share its memory");
 
 // D: head dimension, FMT: type of q and out, W: the scores are written for the weights
 template <int D, int FMT, int NT, bool PAIR, bool W>
@@ -158,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
   using Ge = Geo<D, NT, PAIR>;
   using Sm = Smem<D, NT, PAIR>;
   static_assert(!PAIR || (NT == 1 && L::kGroups == 2));
-  constexpr int G = Ge::G, kRows = Ge::kRows;
+  constexpr int G = Ge::G, kRows = Ge::kRows, kSub = Ge::kSub;
   constexpr int GL = PAIR ? 1 : G;               // groups of channels that a lane's columns stand for
   extern __shared__ __align__(16) uint8_t smem_raw[];
   Sm& sm = *reinterpret_cast<Sm*>(smem_raw);
@@ -305,7 +309,6 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
   // ------------------------------ products and softmax ------------------------------
   const int g8 = lane >> 2, t4 = lane & 3;
   const int own = PAIR ? t4 >> 1 : 0;             // PAIR: the group of this lane's columns
-  const int sub = warp / (kWarps / kSub), token0 = (warp % (kWarps / kSub)) * kItem;   // this warp's block of a stage, and its tokens there
   auto row_of = [&](int nt, int c) { return PAIR ? 2 * (t4 & 1) + c : nt * 8 + 2 * t4 + c; };   // row of the unit that a lane's column stands for
   bool ok = true;
   for (;; ++parts) {
@@ -606,23 +609,46 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
       const uint32_t stage = step % Ge::kStages;
       ok = ptx::mbar_wait(&sm.full[stage], (step / Ge::kStages) & 1u, p.timeout_ns, abort_flag);
       if (!ok) break;
-      if (i + sub < part.i1) {
-        const int key0 = span.block(i + sub) * kPage + token0;
-        const uint8_t* block = sm.stage[stage][sub];
-        if (key0 + kItem - 1 <= pos_lo && (p.window == 0 || pos_hi - key0 < p.window || key0 + kItem <= p.sinks)) {
-          // (two tiles at once where their state fits the registers)
-          if constexpr (PAIR || (NT == 1 && G == 1)) {
-            tiles(std::true_type{}, std::integral_constant<int, kItem / kTile>{}, block, token0, key0);
+      // Tiles that all rows see whole go several at once, as their state fits the registers; the others by themselves
+      auto whole = [&](int key0, int n) {
+        const int behind = key0 + n * kTile;
+        return behind - 1 <= pos_lo && (p.window == 0 || pos_hi - key0 < p.window || behind <= p.sinks);
+      };
+      auto masked = [&](const uint8_t* block, int t0, int key0) {
+        if (key0 <= pos_hi && (p.window == 0 || pos_lo - (key0 + kTile - 1) < p.window || key0 < p.sinks))
+          tiles(std::false_type{}, std::integral_constant<int, 1>{}, block, t0, key0);
+      };
+      const int count = min(kSub, part.i1 - i);
+      if constexpr (NT == 2) {
+        // (half a block a warp)
+        const int at = warp / 2, t0 = warp % 2 * 2 * kTile;
+        if (at < count) {
+          const int key0 = span.block(i + at) * kPage + t0;
+          const uint8_t* block = sm.stage[stage][at];
+          if (whole(key0, 2)) {
+#pragma unroll 1
+            for (int t = 0; t < 2 * kTile; t += kTile) tiles(std::true_type{}, std::integral_constant<int, 1>{}, block, t0 + t, key0 + t);
           } else {
 #pragma unroll 1
-            for (int t = 0; t < kItem; t += kTile) tiles(std::true_type{}, std::integral_constant<int, 1>{}, block, token0 + t, key0 + t);
+            for (int t = 0; t < 2 * kTile; t += kTile) masked(block, t0 + t, key0 + t);
           }
-        } else {
-#pragma unroll 1
-          for (int t = 0; t < kItem; t += kTile) {
-            const int k0 = key0 + t;
-            if (k0 <= pos_hi && (p.window == 0 || pos_lo - (k0 + kTile - 1) < p.window || k0 < p.sinks))
-              tiles(std::false_type{}, std::integral_constant<int, 1>{}, block, token0 + t, k0);
+        }
+      } else {
+        // (the tiles of the stage's blocks, as many for each warp)
+        const int end = (warp + 1) * count;
+        for (int t = warp * count; t < end;) {
+          const int at = t / kTilesBlock, t0 = t % kTilesBlock * kTile, key0 = span.block(i + at) * kPage + t0;
+          const uint8_t* block = sm.stage[stage][at];
+          if (Ge::kTiles == 4 && count == 4 && whole(key0, 4)) {
+            tiles(std::true_type{}, std::integral_constant<int, Ge::kTiles>{}, block, t0, key0);
+            t += 4;
+          } else if (count % 2 == 0 && whole(key0, 2)) {
+            tiles(std::true_type{}, std::integral_constant<int, 2>{}, block, t0, key0);
+            t += 2;
+          } else {
+            if (whole(key0, 1)) tiles(std::true_type{}, std::integral_constant<int, 1>{}, block, t0, key0);
+            else masked(block, t0, key0);
+            ++t;
           }
         }
       }
@@ -830,7 +856,7 @@ bool decode_plan(const CatcocKv4Call& c, bool weights, DecodePlan& d) {
   if (d.blocks > (1ll << 30) || static_cast<int64_t>(c.max_pages) * kPage > (1ll << 24)) return false;
   int device = 0;
   cudaGetDevice(&device);
-  d.ctas = static_cast<int>(std::min<int64_t>(d.blocks, static_cast<int64_t>(catcoc_num_sms(device)) * (d.rows == 16 ? 2 : 3)));
+  d.ctas = static_cast<int>(std::min<int64_t>(d.blocks, 2ll * catcoc_num_sms(device)));
   const int64_t pieces = d.ctas + d.units;
   d.o_floats = pieces * d.rows * c.D;
   d.ml_floats = pieces * d.rows * 2;
