@@ -634,15 +634,16 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
           }
         }
       } else {
-        // (the tiles of the stage's blocks, as many for each warp)
+        // (the tiles of the stage's blocks, as many for each warp. Several go at once only from where they end in their block and in this
+        // warp's share: behind the first, masked tiles of a window the walk may stand anywhere.)
         const int end = (warp + 1) * count;
         for (int t = warp * count; t < end;) {
           const int at = t / kTilesBlock, t0 = t % kTilesBlock * kTile, key0 = span.block(i + at) * kPage + t0;
           const uint8_t* block = sm.stage[stage][at];
-          if (Ge::kTiles == 4 && count == 4 && whole(key0, 4)) {
+          if (Ge::kTiles == 4 && count == 4 && t0 == 0 && whole(key0, 4)) {
             tiles(std::true_type{}, std::integral_constant<int, Ge::kTiles>{}, block, t0, key0);
             t += 4;
-          } else if (count % 2 == 0 && whole(key0, 2)) {
+          } else if (count % 2 == 0 && t % 2 == 0 && whole(key0, 2)) {
             tiles(std::true_type{}, std::integral_constant<int, 2>{}, block, t0, key0);
             t += 2;
           } else {
