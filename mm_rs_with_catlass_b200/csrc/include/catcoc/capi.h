@@ -377,7 +377,8 @@ int catcoc_mla_rows(const void* q_nope, const void* q_rope, const void* ckv, con
 
 /* ---- paged key / value cache in 4 bits (csrc/kernels/kv4_cache.cu, kv4_decode.cu; layout: kv4.h) ----
  * cache: uint8 [pages, Hk, catcoc_kv4_block_bytes(D)], 64 tokens of a head a block, D = 64 or 128; block_table [B, max_pages] and
- * kv_lens [B] are device int32. A page outside the cache or a length outside the table's row is noted in `status` and left out.
+ * kv_lens [B] are device int32. A page outside the cache is noted in `status` and left out. So is a length that the table's row cannot hold: append
+ * leaves out the tokens outside of the row, the other functions take the row's whole, or nothing for a negative length.
  * The numbers of a call travel in one block, which a caller may keep; each function reads those that it names. */
 typedef struct CatcocKv4Call {
   int B, Hk, D, pages, max_pages;  /* all */

@@ -37,7 +37,7 @@ CATCOC_DEVICE void note(uint32_t* status, uint32_t what, int seen, int limit) {
   }
 }
 
-// Length of a sequence, within what its row of the block table can hold
+// Length of a sequence, cut to what its row of the block table can hold
 CATCOC_DEVICE int seq_len(const int* lens, int b, int capacity, uint32_t* status) {
   const int n = lens[b];
   if (n < 0 || n > capacity) {

@@ -174,9 +174,11 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(const AppendParams p) {
     exchange(vw);
   }
   if (!real || b >= p.B || behind <= 0) return;           // a token behind the last sequence
-  const int len = seq_len(p.lens, b, p.max_pages * kPage, p.status);
-  const int pos = len - behind;
-  if (pos < 0) { if (j == 0) note(p.status, kErrLen, len, behind); return; }
+  // (from the length as it is: counted from one that is cut to the table's row, the token would land on one of the sequence's last)
+  const int len = p.lens[b];
+  const int64_t at_pos = static_cast<int64_t>(len) - behind;
+  if (at_pos < 0 || at_pos >= p.max_pages * kPage) { if (j == 0) note(p.status, kErrLen, len, at_pos < 0 ? behind : p.max_pages * kPage); return; }
+  const int pos = static_cast<int>(at_pos);
   const int page = page_of(p.table, static_cast<int64_t>(b) * p.max_pages, pos / kPage, p.pages, p.status);
   if (page < 0) return;
   uint8_t* block = p.cache + (static_cast<int64_t>(page) * p.Hk + h) * L::kBytes;

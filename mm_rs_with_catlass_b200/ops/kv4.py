@@ -9,8 +9,10 @@ As for :func:`mla_decode`, ``block_table`` ``[B, max_pages]`` (int32) names the 
     out = kv4_decode(q, cache, block_table, kv_lens, weights=sums) # ... attend; `sums` gathers what was attended to
     kept, kv_lens = kv4_evict(cache, sums, block_table, kv_lens, keep, recent=..., sinks=...)   # now and then
 
-and :func:`kv4_read` gives tokens back in 16 bits. A page that is not in the cache, or a length that the table's row cannot
-hold, is left out and noted in the device's status block (``ops._common.raise_on_status``), as a wait that ran out of time is.
+and :func:`kv4_read` gives tokens back in 16 bits. A page that is not in the cache is left out, and noted in the device's status
+block (``ops._common.raise_on_status``), as a wait that ran out of time is. A length that the table's row cannot hold is noted too:
+:func:`kv4_append` leaves out the tokens whose positions lie outside of the row, the other functions take as many tokens as the row holds
+(none for a negative length).
 Every value of a group that holds an infinity or a NaN reads as NaN; what pages hold behind a sequence's
 length, or in front of its window, does not reach a result.
 
