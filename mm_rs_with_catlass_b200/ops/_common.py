@@ -199,6 +199,16 @@ def guard(device: torch.device):
     return _NO_GUARD if on_device(device) else torch.cuda.device(device)
 
 
+def whole(x) -> int:
+    """A number of a call as an int: what calls are kept by holds numbers, never a tensor, which would be known by its identity."""
+    if type(x) is int:
+        return x
+    n = int(x)
+    if n != x:
+        raise TypeError("a whole number is wanted, got %r" % (x,))
+    return n
+
+
 def layout(t: Optional[torch.Tensor]):
     """What an argument block says about a tensor besides its address. Blocks that are kept by the layouts of a call's tensors
     serve any buffers so laid out: the caller writes the addresses into a copy and checks what depends on them."""

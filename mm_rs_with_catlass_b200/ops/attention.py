@@ -97,6 +97,7 @@ _windows: dict = {}
 
 def _windowed(q, k, v, causal, scale, out, window, sinks):
     lay = cm.layout
+    causal, window, sinks, scale = bool(causal), cm.whole(window), cm.whole(sinks), None if scale is None else float(scale)
     key = (lay(q), lay(k), lay(v), lay(out), causal, scale, window, sinks)
     plan = _windows.get(key)
     if plan is None:
@@ -127,10 +128,10 @@ def _window_plan(q, k, v, causal, scale, out, window, sinks):
         raise ValueError("the window must be at least 1 and sinks not negative (got %d and %d)" % (window, sinks))
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
         raise ValueError("out must be a contiguous tensor shaped like q")
-    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
     if not scale > 0.0:
         raise ValueError("the softmax scale must be positive")
-    window, sinks = min(int(window), 1 << 30), min(int(sinks), 1 << 30)
+    window, sinks = min(window, 1 << 30), min(sinks, 1 << 30)
     with cm.guard(dev):
         need = int(N.lib().catcoc_window_route(b, hq, hk, sq, sk, d, window, sinks))
     need = need if need >= 0 else -1 - need

@@ -167,6 +167,7 @@ def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tens
     ``start[b] + count - 1`` (``start`` ``[B]``, int32; from the beginning without it; ``count``: as many as the table's
     row can hold), zero where a sequence has no token."""
     lay = cm.layout
+    count = None if count is None else cm.whole(count)
     key = (1, lay(cache), lay(block_table), lay(kv_lens), lay(start), count, dtype)
     plan = _plans.get(key)
     if plan is None:
@@ -176,7 +177,7 @@ def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tens
         if dtype not in _FMT:
             raise TypeError("kv4_read gives fp16 / bf16")
         _device_ints(start, "start", batch)
-        n = width * PAGE if count is None else int(count)
+        n = width * PAGE if count is None else count
         if n < 1:
             raise ValueError("count must be positive")
         plan = _keep(key, _Plan(dev, B=batch, Hk=heads, D=d, pages=pages, max_pages=width, fmt=_FMT[dtype], count=n))
@@ -200,6 +201,7 @@ def kv4_decode(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, 
     gives zeros.
     """
     lay = cm.layout
+    q_len, sinks, window, scale = cm.whole(q_len), cm.whole(sinks), None if window is None else cm.whole(window), None if scale is None else float(scale)
     key = (2, lay(q), lay(cache), lay(block_table), lay(kv_lens), lay(weights), lay(out), q_len, window, sinks, scale)
     plan = _plans.get(key)
     if plan is None:
@@ -244,7 +246,7 @@ def _decode_plan(q, cache, block_table, kv_lens, q_len, window, sinks, weights, 
     if out is not None and (out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous()):
         raise ValueError("out must be a contiguous tensor shaped like q")
     plan = _Plan(dev, not q.is_contiguous(), B=batch, Hk=heads, D=d, pages=pages, max_pages=width, fmt=_FMT[q.dtype], Hq=hq, q_len=q_len,
-                 window=min(int(window), 1 << 30), sinks=min(int(sinks), 1 << 30), scale=float(scale), S=weights.shape[2] if weights is not None else 0)
+                 window=min(window, 1 << 30), sinks=min(sinks, 1 << 30), scale=scale, S=weights.shape[2] if weights is not None else 0)
     with cm.guard(dev):
         need = int(N.lib().catcoc_kv4_decode_workspace_bytes(plan.at, int(weights is not None)))
     if need < 0:
@@ -266,13 +268,13 @@ def kv4_evict(cache: torch.Tensor, weights: torch.Tensor, block_table: torch.Ten
     ``min(kv_lens, keep)`` as a new int32 tensor. ``block_table`` and ``kv_lens`` are not changed.
     """
     lay = cm.layout
+    keep, recent, sinks = cm.whole(keep), cm.whole(recent), cm.whole(sinks)
     key = (3, lay(cache), lay(weights), lay(block_table), lay(kv_lens), lay(out_table), lay(out_weights), keep, recent, sinks)
     plan = _plans.get(key)
     if plan is None:
         dev = cm.require_cuda(cache, weights, block_table, kv_lens, out_table, out_weights)
         pages, heads, d = _cache_dims(cache)
         batch, width = _sequences(block_table, kv_lens)
-        keep, recent, sinks = int(keep), int(recent), int(sinks)
         if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
             raise ValueError("keep=%d must be positive and hold the %d first and %d last tokens" % (keep, sinks, recent))
         _weights(weights, batch, heads, width * PAGE)
