@@ -181,9 +181,16 @@ def on_device(device: torch.device) -> bool:
     return _current_device() == (device.index if device.index is not None else 0)
 
 
+def to_keep(t: torch.Tensor) -> torch.Tensor:
+    """``t``, which outlives the call; refused where it has no memory, as under ``FakeTensorMode``: later calls would take it for real."""
+    if type(t) is not torch.Tensor:
+        raise RuntimeError("kernels run on real tensors only; under this mode new tensors are %ss" % type(t).__name__)
+    return t
+
+
 def like(shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     """What :func:`fresh` makes tensors like: a view of one element, to be kept."""
-    return torch.empty(1, dtype=dtype, device=device).expand(shape)
+    return to_keep(torch.empty(1, dtype=dtype, device=device)).expand(shape)
 
 
 def fresh(template: torch.Tensor) -> torch.Tensor:
@@ -342,7 +349,7 @@ def local_status(device: torch.device) -> torch.Tensor:
     key = (device.type, device.index)
     st = _status_cache.get(key)
     if st is None:
-        st = torch.zeros(8, dtype=torch.int32, device=device)
+        st = to_keep(torch.zeros(8, dtype=torch.int32, device=device))
         _status_cache[key] = st
     return st
 

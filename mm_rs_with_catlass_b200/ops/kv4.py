@@ -86,11 +86,11 @@ _plans: dict = {}
 class _Plan:
     __slots__ = ("call", "at", "device", "status", "fresh", "copy")
 
-    def __init__(self, device, copy=(), **numbers):
+    def __init__(self, device, copy=(), fresh=None, **numbers):
         self.call = N.Kv4Call(**numbers)
         self.at = C.addressof(self.call)
         self.device, self.status = device, cm.local_status(device).data_ptr()
-        self.copy, self.fresh = copy, None         # which operands are copied first; what results or scratch are made like
+        self.copy, self.fresh = copy, fresh        # which operands are copied first; what results or scratch are made like
 
 
 def _keep(key, plan: _Plan) -> _Plan:
@@ -180,8 +180,8 @@ def kv4_read(cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tens
         n = width * PAGE if count is None else count
         if n < 1:
             raise ValueError("count must be positive")
-        plan = _keep(key, _Plan(dev, B=batch, Hk=heads, D=d, pages=pages, max_pages=width, fmt=_FMT[dtype], count=n))
-        plan.fresh = cm.like((batch, heads, n, d), dtype, dev)
+        plan = _keep(key, _Plan(dev, fresh=cm.like((batch, heads, n, d), dtype, dev), B=batch, Hk=heads, D=d, pages=pages, max_pages=width,
+                                fmt=_FMT[dtype], count=n))
     k, v = cm.fresh(plan.fresh), cm.fresh(plan.fresh)
     _run(plan, N.lib().catcoc_kv4_read, cache.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr(), start.data_ptr() if start is not None else None,
          k.data_ptr(), v.data_ptr(), plan.status)
@@ -286,10 +286,10 @@ def kv4_evict(cache: torch.Tensor, weights: torch.Tensor, block_table: torch.Ten
                 raise ValueError("out_table must name pages for %d tokens" % most)
         if out_weights is not None:
             _weights(out_weights, batch, heads, most, "out_weights")
-        plan = _keep(key, _Plan(dev, B=batch, Hk=heads, D=d, pages=pages, max_pages=width, S=weights.shape[2], keep=keep, recent=recent, sinks=sinks,
+        plan = _keep(key, _Plan(dev, fresh=cm.like((batch, heads, keep), torch.int32, dev), B=batch, Hk=heads, D=d, pages=pages, max_pages=width,
+                                S=weights.shape[2], keep=keep, recent=recent, sinks=sinks,
                                 S_out=(weights if out_weights is None else out_weights).shape[2],
                                 out_pages=(block_table if out_table is None else out_table).shape[1]))
-        plan.fresh = cm.like((batch, heads, keep), torch.int32, dev)
     kept, lens = cm.fresh(plan.fresh), torch.empty_like(kv_lens)
     _run(plan, N.lib().catcoc_kv4_evict, cache.data_ptr(), weights.data_ptr(), (weights if out_weights is None else out_weights).data_ptr(),
          block_table.data_ptr(), (block_table if out_table is None else out_table).data_ptr(), kv_lens.data_ptr(), kept.data_ptr(), lens.data_ptr(),
