@@ -349,7 +349,8 @@ def local_status(device: torch.device) -> torch.Tensor:
     key = (device.type, device.index)
     st = _status_cache.get(key)
     if st is None:
-        st = to_keep(torch.zeros(8, dtype=torch.int32, device=device))
+        with torch.inference_mode(False):            # (raise_on_status clears it, from wherever it is called)
+            st = to_keep(torch.zeros(8, dtype=torch.int32, device=device))
         _status_cache[key] = st
     return st
 
