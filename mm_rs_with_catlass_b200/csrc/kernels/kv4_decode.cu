@@ -634,16 +634,18 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
           }
         }
       } else {
-        // (the tiles of the stage's blocks, as many for each warp. Several go at once only from where they end in their block and in this
-        // warp's share: behind the first, masked tiles of a window the walk may stand anywhere.)
+        // The tiles of the stage's blocks, as many for each warp. Several go at once only from where they end in their block and in this
+        // warp's share: behind the first, masked tiles of a window the walk may stand anywhere. (Both numbers in one test: as two, D = 64 takes
+        // 19.9 us instead of 18.6 for 16 x 8 heads x 4096 tokens.)
         const int end = (warp + 1) * count;
         for (int t = warp * count; t < end;) {
           const int at = t / kTilesBlock, t0 = t % kTilesBlock * kTile, key0 = span.block(i + at) * kPage + t0;
           const uint8_t* block = sm.stage[stage][at];
-          if (Ge::kTiles == 4 && count == 4 && t0 == 0 && whole(key0, 4)) {
+          const int most = (t | count) & 3;
+          if (Ge::kTiles == 4 && most == 0 && whole(key0, 4)) {
             tiles(std::true_type{}, std::integral_constant<int, Ge::kTiles>{}, block, t0, key0);
             t += 4;
-          } else if (count % 2 == 0 && t % 2 == 0 && whole(key0, 2)) {
+          } else if ((most & 1) == 0 && whole(key0, 2)) {
             tiles(std::true_type{}, std::integral_constant<int, 2>{}, block, t0, key0);
             t += 2;
           } else {
