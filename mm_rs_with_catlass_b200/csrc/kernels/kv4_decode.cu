@@ -150,6 +150,7 @@ struct Smem {
   float2 ml[kWarps][Ge::kRows];
   alignas(16) uint16_t q[2][Ge::kRows * D];   // the rows of a part, and of the one behind it
   Part part[2];                        // n = 0: the run is at its end
+  uint32_t there[Ge::kStages];         // which of a stage's blocks are in the cache, a bit each
   uint64_t full[Ge::kStages], empty[Ge::kStages], part_full[2], part_empty[2];
   uint32_t abort_flag, failed[kWarps];
 };
@@ -255,12 +256,14 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
       at += part.i1 - part.i0;
       Part next = part;
       int ids = -1, next_raw = 0;
+      uint32_t named = 0;
       for (int i = part.i0; i < part.i1; i += kSub, ++step) {
-        // the names of 32 blocks at a time, so that no copy waits for its own
         const int k = (i - part.i0) & 31;
+        // the names of 32 blocks at a time, so that no copy waits for its own (one that is not in the cache is noted, and left out by the consumers)
         if (k == 0) {
           if (i > part.i0) raw = names(part, i);
           ids = i + lane < part.i1 ? checked_page(raw, p.pages, p.status) : -1;
+          named = __ballot_sync(0xffffffffu, ids >= 0);
         }
         const uint32_t stage = step % Ge::kStages;
         ok = ptx::mbar_wait(&sm.empty[stage], ((step / Ge::kStages) & 1u) ^ 1u, p.timeout_ns, abort_flag);
@@ -272,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
           found += page[s] >= 0;
         }
         if (lane == 0) {
-          // (a block that is not in the cache was noted: what the stage held stands in for it)
+          sm.there[stage] = named >> k;
           if (found == 0) ptx::mbar_arrive(&sm.full[stage]);
           else ptx::mbar_expect_tx(&sm.full[stage], static_cast<uint32_t>(found * L::kBytes));
 #pragma unroll
@@ -618,12 +621,15 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
         if (key0 <= pos_hi && (p.window == 0 || pos_lo - (key0 + kTile - 1) < p.window || key0 < p.sinks))
           tiles(std::false_type{}, std::integral_constant<int, 1>{}, block, t0, key0);
       };
+      // First key of a tile; that of a block that is not in the cache lies behind all that any row sees, and the block is left out
+      const uint32_t there = sm.there[stage];
+      auto first_key = [&](int at, int t0) { return (there >> at) & 1u ? span.block(i + at) * kPage + t0 : 1 << 30; };
       const int count = min(kSub, part.i1 - i);
       if constexpr (NT == 2) {
         // (half a block a warp)
         const int at = warp / 2, t0 = warp % 2 * 2 * kTile;
         if (at < count) {
-          const int key0 = span.block(i + at) * kPage + t0;
+          const int key0 = first_key(at, t0);
           const uint8_t* block = sm.stage[stage][at];
           if (whole(key0, 2)) {
 #pragma unroll 1
@@ -639,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, Geo<D, NT, PAIR>::kCtas) kv4_decode_
         // 19.9 us instead of 18.6 for 16 x 8 heads x 4096 tokens.)
         const int end = (warp + 1) * count;
         for (int t = warp * count; t < end;) {
-          const int at = t / kTilesBlock, t0 = t % kTilesBlock * kTile, key0 = span.block(i + at) * kPage + t0;
+          const int at = t / kTilesBlock, t0 = t % kTilesBlock * kTile, key0 = first_key(at, t0);
           const uint8_t* block = sm.stage[stage][at];
           const int most = (t | count) & 3;
           if (Ge::kTiles == 4 && most == 0 && whole(key0, 4)) {
@@ -810,12 +816,14 @@ __global__ void __launch_bounds__(256) kv4_weights_kernel(const DecodeParams p, 
   const int len = min(max(p.lens[b], 0), p.max_pages * kPage);
   const int j = blockIdx.y * 256 + threadIdx.x;
   if (static_cast<int>(blockIdx.y) * 256 >= len) return;
+  // (what is not in the cache has no scores)
+  const bool there = j < len && static_cast<uint32_t>(p.table[static_cast<int64_t>(b) * p.max_pages + j / kPage]) < static_cast<uint32_t>(p.pages);
   for (int r = threadIdx.x; r < p.R; r += 256) {
     const float2 ml = *reinterpret_cast<const float2*>(p.row_ml + (static_cast<int64_t>(bh) * p.R + r) * 2);
     row[r] = make_float2(ml.x == -INFINITY ? 0.0f : ml.x, ml.y == 0.0f ? 0.0f : 1.0f / ml.y);
   }
   __syncthreads();
-  if (j >= len) return;
+  if (!there) return;
   const float* s = p.scores + static_cast<int64_t>(bh) * p.R * p.S + j;
   float sum = 0.0f;
 #pragma unroll 4

@@ -84,12 +84,12 @@ def _without(q, cache, table, kv_lens, there, q_len, window, sinks):
 
 @pytest.mark.parametrize("window,sinks", [(None, 0), (900, 70)])
 @pytest.mark.parametrize("d,group,q_len", [(128, 4, 1), (128, 8, 1), (128, 16, 1), (64, 3, 2), (64, 16, 1)])
-@pytest.mark.parametrize("many", [False, True])
-def test_decode_leaves_out_what_is_not_in_the_cache(d, group, q_len, window, sinks, many):
+@pytest.mark.parametrize("kind", ["few", "many", "long"])
+def test_decode_leaves_out_what_is_not_in_the_cache(d, group, q_len, window, sinks, kind):
     """Attention is that over the other pages' tokens, and their weights alone change; stages of which some blocks or all are missing, sequences
     without the first page, the last, or any. What the missing blocks' places in shared memory held before does not show."""
-    lens = [2100 - 97 * i for i in range(16)] if many else [700, 300, 64, 333, 190, 77, 1, 500]
-    heads = 4 if many else 1
+    lens = {"many": [2100 - 97 * i for i in range(16)], "few": [700, 300, 64, 333, 190, 77, 1, 500], "long": [45000, 44001, 64, 333, 190, 77, 1, 500]}[kind]
+    heads = {"many": 4, "few": 1, "long": 8}[kind]            # (long: runs of more than 32 blocks, whose names come 32 at a time)
     cache, table, kv_lens, k, v, ends, g = _make(lens, heads, d, seed=group, extra=1)
     catcoc.kv4_append(cache, k, v, table, kv_lens, ends=ends)
     there = torch.rand(table.shape, device=DEV, generator=g) > 0.15
