@@ -446,11 +446,12 @@ static int decode_call(const void* q, const void* k, const void* v, void* out, v
     set_error("flash_decode: bad arguments");
     return CATCOC_E_BAD_ARG;
   }
-  if (reinterpret_cast<uintptr_t>(out) & 15) { set_error("attention operands must be 16-byte aligned"); return CATCOC_E_ALIGNMENT; }
+  const DecodePlan d = decode_plan(B, Hq, Hk, Sq, Sk, device_sms(), window, sinks);
+  // A CTA that has a whole sequence stores its rows 16 bytes at a time, the merge of those that are cut 4; with runs shorter than a sequence all are cut.
+  if (reinterpret_cast<uintptr_t>(out) & (d.per < d.nb ? 3 : 15)) { set_error("attention operands must be 16-byte aligned"); return CATCOC_E_ALIGNMENT; }
   if (fmt != CATCOC_FMT_F16 && fmt != CATCOC_FMT_BF16) { set_error("flash_attention takes fp16 / bf16"); return CATCOC_E_UNSUPPORTED; }
   if (causal && Sk < Sq) { set_error("causal attention needs Sk >= Sq"); return CATCOC_E_BAD_ARG; }
   if (!(scale > 0.0f)) { set_error("flash_attention: the softmax scale must be positive (the row maximum is taken before scaling)"); return CATCOC_E_UNSUPPORTED; }
-  const DecodePlan d = decode_plan(B, Hq, Hk, Sq, Sk, device_sms(), window, sinks);
   decode::DecodeParams p;
   memset(&p, 0, sizeof(p));
   const CUtensorMapDataType dt = fmt == CATCOC_FMT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
