@@ -814,8 +814,8 @@ __global__ void __launch_bounds__(256) kv4_weights_kernel(const DecodeParams p, 
   ptx::grid_dependency_wait();
   const int bh = blockIdx.x, b = bh / p.Hk;
   const int len = min(max(p.lens[b], 0), p.max_pages * kPage);
-  const int j = blockIdx.y * 256 + threadIdx.x;
-  if (static_cast<int>(blockIdx.y) * 256 >= len) return;
+  const int j0 = static_cast<int>(blockIdx.z * gridDim.y + blockIdx.y) * 256, j = j0 + threadIdx.x;   // (2^24 tokens are 65536 blocks, one more than grid y has)
+  if (j0 >= len) return;
   // (what is not in the cache has no scores)
   const bool there = j < len && static_cast<uint32_t>(p.table[static_cast<int64_t>(b) * p.max_pages + j / kPage]) < static_cast<uint32_t>(p.pages);
   for (int r = threadIdx.x; r < p.R; r += 256) {
@@ -918,9 +918,11 @@ extern "C" int catcoc_kv4_decode(const CatcocKv4Call* c, const void* q, const vo
     CATCOC_CUDA_OK(launch_overlapped(main_kernel, dim3(static_cast<unsigned>(d.ctas)), dim3(kThreads), smem, stream, p));
     CATCOC_CUDA_OK(launch_overlapped(combine_kernel, dim3(static_cast<unsigned>(d.units), static_cast<unsigned>((std::min(d.R, d.rows) + 3) / 4)), dim3(128), 0,
                                      stream, p, d.rows, d.ctas));
-    if (weights)
-      CATCOC_CUDA_OK(launch_overlapped(kv4_weights_kernel, dim3(static_cast<unsigned>(B * Hk), static_cast<unsigned>((p.S + 255) / 256)), dim3(256),
-                                       d.R * sizeof(float2), stream, p, weights, static_cast<int64_t>(c->S)));
+    if (weights) {
+      const unsigned chunks = static_cast<unsigned>((p.S + 255) / 256), y = std::min(chunks, 32768u);
+      CATCOC_CUDA_OK(launch_overlapped(kv4_weights_kernel, dim3(static_cast<unsigned>(B * Hk), y, (chunks + y - 1) / y), dim3(256), d.R * sizeof(float2), stream, p,
+                                       weights, static_cast<int64_t>(c->S)));
+    }
     return CATCOC_OK;
   };
   auto by_rows = [&](auto dim, auto type) -> int {
