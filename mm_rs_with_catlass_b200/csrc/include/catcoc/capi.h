@@ -402,7 +402,7 @@ int catcoc_kv4_read(const CatcocKv4Call* c, const void* cache, const int* block_
                     uint32_t* status, void* stream);
 /* Cuts every sequence to its first `sinks`, last `recent` and, of the others, heaviest tokens (the first ones of equal weight), `keep`
  * in all, in order. kept [B, Hk, keep] (-1 behind the last), out_lens [B], out_weights [B, Hk, S_out] (zero behind the last).
- * In place when out_table is block_table. Two launches. */
+ * In place when out_table is block_table. One launch, or two where few heads (less than half as many as SMs) move more than 1024 tokens to other pages. */
 int catcoc_kv4_evict(const CatcocKv4Call* c, void* cache, const float* weights, float* out_weights, const int* block_table, const int* out_table,
                      const int* kv_lens, int* kept, int* out_lens, uint32_t* status, void* stream);
 /* Attention of q_len new tokens of every sequence (q, out [B * q_len, Hq, D]); token t sees the keys up to its own, with window > 0 of

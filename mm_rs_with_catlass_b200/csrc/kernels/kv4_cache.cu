@@ -551,9 +551,11 @@ extern "C" int catcoc_kv4_evict(const CatcocKv4Call* c, void* cache, const float
     CATCOC_CUDA_OK(launch_overlapped(kernel, grid, dim3(static_cast<unsigned>(threads)), 0, stream, p));
     return CATCOC_OK;
   };
-  // One launch where the heads fill most of the SMs or have little to move, and in place, where a head's moves are in order anyway.
+  // One launch where the heads fill half of the SMs or have little to move, and in place, where a head's moves are in order anyway.
   const dim3 grid(static_cast<unsigned>(heads));
-  if (in_place || heads >= 74 || most <= 1024)
+  int device = 0;
+  cudaGetDevice(&device);
+  if (in_place || 2 * heads >= catcoc_num_sms(device) || most <= 1024)
     return c->D == 128 ? launch(kv4_evict_kernel<128, true>, grid, kPickThreads) : launch(kv4_evict_kernel<64, true>, grid, kPickThreads);
   const int first = c->D == 128 ? launch(kv4_evict_kernel<128, false>, grid, kPickThreads) : launch(kv4_evict_kernel<64, false>, grid, kPickThreads);
   if (first != CATCOC_OK) return first;

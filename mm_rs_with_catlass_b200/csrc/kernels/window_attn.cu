@@ -512,7 +512,7 @@ struct WindowPlan {
   int slices, per;     // keys cut into slices of `per` blocks
 };
 
-WindowPlan window_plan(int B, int Hq, int Hk, int Sq, int Sk, int window, int sinks) {
+WindowPlan window_plan(int B, int Hq, int Hk, int Sq, int Sk, int window, int sinks, int sms) {
   const int group = Hq / Hk, rows = window::kTiles * window::kBQ, pos = Sq;
   // blocks of the list of `span` positions that end before key `end`, at most (Work: those of the sinks are whole ones)
   auto blocks = [&](int64_t end, int span) {
@@ -526,7 +526,7 @@ WindowPlan window_plan(int B, int Hq, int Hk, int Sq, int Sk, int window, int si
     Form f{{hq, sq, (sq + rows - 1) / rows, 1, 0}, blocks(Sk, span), 0.0};
     double sum = 0.0;
     for (int i = 0; i < f.plan.tiles; ++i) sum += 1.0 + blocks(span == pos ? Sk : std::min<int64_t>(Sk, static_cast<int64_t>(i + 1) * rows + Sk - pos), span);
-    f.load = std::max(1.0 + f.longest, static_cast<double>(B) * hq * sum / 148.0);
+    f.load = std::max(1.0 + f.longest, static_cast<double>(B) * hq * sum / sms);
     return f;
   };
   int n = 1;
@@ -541,13 +541,19 @@ WindowPlan window_plan(int B, int Hq, int Hk, int Sq, int Sk, int window, int si
   for (int f = 0; f < n; ++f) {
     const WindowPlan& x = forms[f].plan;
     const int64_t works = static_cast<int64_t>(B) * x.Hq * x.tiles, out_rows = static_cast<int64_t>(B) * x.Hq * x.Sq;
-    for (int s = 2; s <= 16 && works * s <= 148 && 2 * s <= forms[f].longest; ++s) {
+    for (int s = 2; s <= 16 && works * s <= sms && 2 * s <= forms[f].longest; ++s) {
       const int per = (forms[f].longest + s - 1) / s, slices = (forms[f].longest + per - 1) / per;
       const double us = 9.0 + 1.55 * per + static_cast<double>(slices) * out_rows * 128 * 8 / 3e6;
       if (us < best_us) { best_us = us; best = x; best.slices = slices; best.per = per; }
     }
   }
   return best;
+}
+
+int current_sms() {
+  int device = 0;
+  cudaGetDevice(&device);
+  return catcoc_num_sms(device);
 }
 
 bool window_args(int B, int Hq, int Hk, int Sq, int Sk, int D, int window, int sinks) {
@@ -561,7 +567,7 @@ extern "C" int64_t catcoc_window_route(int B, int Hq, int Hk, int Sq, int Sk, in
   sinks = std::min(sinks, 1 << 30);
   const int64_t decode = catcoc_window_decode_workspace_bytes(B, Hq, Hk, Sq, Sk, D, window, sinks);
   if (decode >= 0) return decode;
-  const WindowPlan d = window_plan(B, Hq, Hk, Sq, Sk, window, sinks);
+  const WindowPlan d = window_plan(B, Hq, Hk, Sq, Sk, window, sinks, current_sms());
   return -1 - (d.slices > 1 ? static_cast<int64_t>(d.slices) * B * Hq * Sq * (D + 2) * static_cast<int64_t>(sizeof(float)) : 0);
 }
 
@@ -578,7 +584,8 @@ extern "C" int catcoc_window_attention(const void* q, const void* k, const void*
   if (catcoc_window_decode_workspace_bytes(B, Hq, Hk, Sq, Sk, D, window, sinks) >= 0)
     return catcoc_window_decode(q, k, v, out, workspace, B, Hq, Hk, Sq, Sk, D, fmt, window, sinks, scale, status, timeout_ns, stream_);
   const int pos = Sq;
-  const WindowPlan d = window_plan(B, Hq, Hk, Sq, Sk, window, sinks);
+  const int sms = current_sms();
+  const WindowPlan d = window_plan(B, Hq, Hk, Sq, Sk, window, sinks, sms);
   if (d.slices > 1 && workspace == nullptr) { set_error("window_attention: no workspace"); return CATCOC_E_BAD_ARG; }
   Hq = d.Hq;
   Sq = d.Sq;
@@ -608,10 +615,8 @@ extern "C" int catcoc_window_attention(const void* q, const void* k, const void*
   p.idesc_pv = ptx::make_instr_desc(1u, f, f, 0u, 1u, 128u, static_cast<uint32_t>(D));
   p.status = status;
   p.timeout_ns = timeout_ns ? timeout_ns : 10000000000ull;
-  int device = 0;
-  cudaGetDevice(&device);
   cudaStream_t stream = static_cast<cudaStream_t>(stream_);
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(works * d.slices, catcoc_num_sms(device))));
+  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(works * d.slices, sms)));
   const int db = D / 64, slots = D == 128 ? 4 : 8;
   const size_t smem = static_cast<size_t>(window::kTiles * db + slots * db) * window::kBlockBytes + window::kOutBytes + sizeof(window::Bars) + 1024;
   auto launch = [&](auto kernel) -> int {
