@@ -31,6 +31,7 @@ from . import _common as cm
 
 PAGE = 64
 GROUP = 64
+_MOST = 0x7fffffff                    # the library's numbers have 32 bits
 _FMT = {torch.float16: N.FMT_F16, torch.bfloat16: N.FMT_BF16}
 
 
@@ -74,6 +75,8 @@ def _device_ints(t: Optional[torch.Tensor], name: str, batch: int) -> None:
 def _weights(weights: torch.Tensor, batch: int, heads: int, tokens: int, what: str = "weights") -> None:
     if weights.dtype != torch.float32 or weights.dim() != 3 or tuple(weights.shape[:2]) != (batch, heads) or not weights.is_contiguous():
         raise ValueError("%s must be a contiguous fp32 tensor [%d, %d, tokens]" % (what, batch, heads))
+    if weights.shape[2] > _MOST:
+        raise ValueError("%s: %d tokens a head are more than the kernels count" % (what, weights.shape[2]))
     if weights.shape[2] < tokens:
         raise ValueError("%s must have room for %d tokens, as the block table has (got %d)" % (what, tokens, weights.shape[2]))
 
@@ -275,6 +278,8 @@ def kv4_evict(cache: torch.Tensor, weights: torch.Tensor, block_table: torch.Ten
         dev = cm.require_cuda(cache, weights, block_table, kv_lens, out_table, out_weights)
         pages, heads, d = _cache_dims(cache)
         batch, width = _sequences(block_table, kv_lens)
+        if keep > _MOST:
+            raise ValueError("keep=%d is more than the kernels count" % keep)
         if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
             raise ValueError("keep=%d must be positive and hold the %d first and %d last tokens" % (keep, sinks, recent))
         _weights(weights, batch, heads, width * PAGE)

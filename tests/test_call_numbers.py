@@ -88,3 +88,14 @@ def test_fractions_are_refused(entries):
     assert entries.seen[-1]["window"] == 2
 
 
+
+
+def test_numbers_of_more_than_32_bits_are_refused(entries):
+    """The library's numbers have 32 bits: 2^32 + 5 would arrive as 5."""
+    from types import SimpleNamespace
+    with pytest.raises(ValueError):
+        _calls()["evict"](keep=(1 << 32) + 5)
+    assert not entries.seen
+    long = SimpleNamespace(dtype=torch.float32, dim=lambda: 3, shape=(1, 1, (1 << 32) + 64), is_contiguous=lambda: True)
+    with pytest.raises(ValueError):
+        kv4._weights(long, 1, 1, 64)
