@@ -247,6 +247,7 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const ReadParams p) {
 
 // ------------------------------------------------------------- evict -------------------------------------------------------------
 
+constexpr int kMostTokens = 1 << 30;
 constexpr int kPickThreads = 1024, kPickItems = 4, kPickStretch = kPickThreads * kPickItems;
 
 struct EvictParams {
@@ -540,6 +541,8 @@ extern "C" int catcoc_kv4_evict(const CatcocKv4Call* c, void* cache, const float
     return bad("kv4_evict: bad arguments");
   const int64_t capacity = static_cast<int64_t>(c->max_pages) * kPage, heads = static_cast<int64_t>(c->B) * c->Hk;
   if (static_cast<int64_t>(c->recent) + c->sinks > c->keep) return bad("kv4_evict: the first and the last tokens are more than what is kept");
+  // (the kernel steps over tokens, places and weights in int, 4096 and more at a time)
+  if (c->keep > kMostTokens || capacity > kMostTokens || c->S_out > kMostTokens) { set_error("kv4_evict: more than 2^30 tokens"); return CATCOC_E_TOO_LARGE; }
   const int64_t most = std::min<int64_t>(c->keep, capacity);      // tokens that can stay
   if (c->S < capacity || static_cast<int64_t>(c->out_pages) * kPage < most || c->S_out < most) return bad("kv4_evict: the weights or the new pages are too short");
   if (unaligned(cache)) { set_error("kv4_evict: the cache must be 16-byte aligned"); return CATCOC_E_ALIGNMENT; }

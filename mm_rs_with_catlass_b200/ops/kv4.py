@@ -278,8 +278,8 @@ def kv4_evict(cache: torch.Tensor, weights: torch.Tensor, block_table: torch.Ten
         dev = cm.require_cuda(cache, weights, block_table, kv_lens, out_table, out_weights)
         pages, heads, d = _cache_dims(cache)
         batch, width = _sequences(block_table, kv_lens)
-        if keep > _MOST:
-            raise ValueError("keep=%d is more than the kernels count" % keep)
+        if keep > 1 << 30:
+            raise ValueError("keep=%d is more than the kernels count (2^30)" % keep)
         if keep < 1 or recent < 0 or sinks < 0 or recent + sinks > keep:
             raise ValueError("keep=%d must be positive and hold the %d first and %d last tokens" % (keep, sinks, recent))
         _weights(weights, batch, heads, width * PAGE)

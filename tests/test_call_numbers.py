@@ -99,3 +99,16 @@ def test_numbers_of_more_than_32_bits_are_refused(entries):
     long = SimpleNamespace(dtype=torch.float32, dim=lambda: 3, shape=(1, 1, (1 << 32) + 64), is_contiguous=lambda: True)
     with pytest.raises(ValueError):
         kv4._weights(long, 1, 1, 64)
+
+
+def test_the_library_refuses_what_its_loops_cannot_count():
+    """Eviction steps over places and weights in int: past 2^30 of them it is refused, before any launch."""
+    import ctypes
+    numbers = dict(B=1, Hk=1, D=64, pages=4, max_pages=2, fmt=N.FMT_BF16, keep=100, recent=2, sinks=2, out_pages=2, S=128, S_out=128)
+
+    def evict(**changes):
+        call = N.Kv4Call(**{**numbers, **changes})
+        return N.lib().catcoc_kv4_evict(ctypes.addressof(call), *[16] * 9, None)
+    assert evict(keep=(1 << 30) + 1) == N.E_TOO_LARGE and evict(keep=0x7fffffff) == N.E_TOO_LARGE
+    assert evict(S_out=0x7fffffff) == N.E_TOO_LARGE
+    assert evict(max_pages=(1 << 24) + 1, S=0x7fffffff) == N.E_TOO_LARGE
